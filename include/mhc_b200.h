@@ -336,6 +336,67 @@ MHC_API int mhc_qlinear_bwd_dx_t(const void* dy, int dy_dtype, const uint32_t* w
                                  int64_t M, int N, int K, int group_size, int bits,
                                  void* stream);
 
+/* ---- losses on logits, with their gradients ---------------------------------
+ * No counterpart in the reference: the losses that a rewired model is tuned
+ * with.  Row t of the logits (bf16, fp16 or fp32) starts at element
+ * (t / rows_per_batch) batch_stride + (t % rows_per_batch) row_stride and has
+ * V contiguous values; targets[t] is its class, or ignore_index for a row that
+ * takes no part.  A target outside [0, V) and a row without a finite logit
+ * give NaN.  logp[t] = ln softmax(x_t)[targets[t]] (0 where ignored);
+ * stats[t] = (max, 1 / sum exp(x - max), 1 - p of the target, 0), four floats
+ * a row (16-byte aligned), for mhc_logits_grad.  rows < 2^28.
+ *   mhc_token_logprobs: logp and stats.
+ *   mhc_logits_grad: dlogits[t, v] = c_t (1[v = targets[t]] - softmax(x_t)[v]),
+ *     c_t = coef[t] * scale * (scale_ptr ? *scale_ptr : 1); dlogits [rows, V]
+ *     contiguous, in the logits' type.  With unless_one, nothing is written
+ *     where *scale_ptr is 1. */
+MHC_API int mhc_token_logprobs(const void* logits, int dtype, int64_t rows,
+                               int64_t rows_per_batch, int64_t batch_stride, int64_t row_stride,
+                               int64_t V, const int64_t* targets, int64_t ignore_index,
+                               float* logp, float* stats, void* stream);
+MHC_API int mhc_logits_grad(const void* logits, int dtype, int64_t rows, int64_t rows_per_batch,
+                            int64_t batch_stride, int64_t row_stride, int64_t V,
+                            const int64_t* targets, int64_t ignore_index, const float* stats,
+                            const float* coef, float scale, const float* scale_ptr,
+                            int unless_one, void* dlogits, void* stream);
+
+/* Paired preference loss.  Sequence s holds rows [cu_seqlens[s],
+ * cu_seqlens[s + 1]) (int32, or int64 with cu_is64; NULL: uniform_len rows
+ * each); sequences 2b and 2b + 1 are pair b's chosen and rejected answers.
+ *   R_s = sum of logp - ref_logp over the sequence's tokens that count,
+ *   z_b = beta (R_2b - R_2b+1)                          -> margins[pairs]
+ *   loss = inv_denominator sum_b (1 - e) softplus(-z_b) + e softplus(z_b),
+ *   e = label_smoothing                                 -> loss[1]
+ * coef[rows] receives d loss / d logp; dlogits (nullable) the gradient times
+ * grad_scale.  Sums over tokens and pairs are fp64, in a fixed order. */
+MHC_API int mhc_preference_loss(const void* logits, int dtype, int64_t rows,
+                                int64_t rows_per_batch, int64_t batch_stride, int64_t row_stride,
+                                int64_t V, const int64_t* targets, int64_t ignore_index,
+                                const void* cu_seqlens, int cu_is64, int64_t uniform_len,
+                                int64_t pairs, const float* ref_logp, float beta,
+                                float label_smoothing, float inv_denominator, float grad_scale,
+                                float* logp, float* stats, float* coef, float* margins,
+                                float* loss, void* dlogits, void* stream);
+
+/* Clipped policy loss with a KL term, per token that counts:
+ *   r = exp(logp - old_logp), k = expm1(ref_logp - logp) - (ref_logp - logp),
+ *   loss = inv_denominator sum_t kl_coef k_t
+ *          - min(r_t A_t, clip(r_t, 1 - clip_low, 1 + clip_high) A_t)
+ * and kl = inv_denominator sum_t k_t (0 without ref_logp, which may be NULL).
+ * inv_denominator 0: one over the number of tokens that count (no such token:
+ * loss, kl and gradient are 0).  coef and dlogits as above.
+ * Workspace (16-byte aligned):
+ * mhc_policy_workspace_bytes() on the current device. */
+MHC_API size_t mhc_policy_workspace_bytes(void);
+MHC_API int mhc_policy_loss(const void* logits, int dtype, int64_t rows, int64_t rows_per_batch,
+                            int64_t batch_stride, int64_t row_stride, int64_t V,
+                            const int64_t* targets, int64_t ignore_index, const float* old_logp,
+                            const float* advantages, const float* ref_logp, float clip_low,
+                            float clip_high, float kl_coef, float inv_denominator,
+                            float grad_scale, float* logp, float* stats, float* coef,
+                            float* loss, float* kl, void* dlogits, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -520,4 +520,95 @@ int mhc_residual_add_agg_bwd(const void* out, int out_dtype, const void* d_out, 
   MHC_TRY_END
 }
 
+// ---- losses on logits ----
+static int check_logits(const char* fn, const LogitsArg& l) {
+  MHC_CHK(check_dtype(fn, "logits", l.dtype));
+  MHC_REQ(l.rows >= 0 && l.rows < ((int64_t)1 << 28), "%s: rows=%lld must be in [0, 2^28)", fn, (long long)l.rows);
+  MHC_REQ(l.vocab >= 1 && l.vocab < ((int64_t)1 << 31), "%s: V=%lld must be in [1, 2^31)", fn, (long long)l.vocab);
+  MHC_REQ(l.per_batch >= 1, "%s: rows_per_batch=%lld must be positive", fn, (long long)l.per_batch);
+  MHC_REQ(l.rows == 0 || (l.logits && l.targets), "%s: NULL logits/targets", fn);
+  const uintptr_t size = (uintptr_t)dtype_size(l.dtype);
+  MHC_REQ(reinterpret_cast<uintptr_t>(l.logits) % size == 0, "%s: logits are not aligned to their type", fn);
+  return MHC_OK;
+}
+
+int mhc_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t rows_per_batch,
+                       int64_t batch_stride, int64_t row_stride, int64_t V, const int64_t* targets,
+                       int64_t ignore_index, float* logp, float* stats, void* stream) {
+  MHC_TRY_BEGIN
+  const LogitsArg l = {logits, dtype, rows, rows_per_batch, batch_stride, row_stride, V, targets, ignore_index};
+  MHC_CHK(check_logits(__func__, l));
+  MHC_REQ(rows == 0 || (logp && stats), "%s: NULL logp/stats", __func__);
+  MHC_REQ(aligned16(stats), "%s: stats must be 16-byte aligned", __func__);
+  return launch_token_logprobs(l, logp, stats, as_stream(stream));
+  MHC_TRY_END
+}
+
+int mhc_logits_grad(const void* logits, int dtype, int64_t rows, int64_t rows_per_batch,
+                    int64_t batch_stride, int64_t row_stride, int64_t V, const int64_t* targets,
+                    int64_t ignore_index, const float* stats, const float* coef, float scale,
+                    const float* scale_ptr, int unless_one, void* dlogits, void* stream) {
+  MHC_TRY_BEGIN
+  const LogitsArg l = {logits, dtype, rows, rows_per_batch, batch_stride, row_stride, V, targets, ignore_index};
+  MHC_CHK(check_logits(__func__, l));
+  MHC_REQ(rows == 0 || (stats && coef && dlogits), "%s: NULL stats/coef/dlogits", __func__);
+  MHC_REQ(!unless_one || scale_ptr, "%s: unless_one needs scale_ptr", __func__);
+  MHC_REQ(aligned16(stats), "%s: stats must be 16-byte aligned", __func__);
+  return launch_logits_grad(l, stats, coef, scale, scale_ptr, unless_one, dlogits, as_stream(stream));
+  MHC_TRY_END
+}
+
+int mhc_preference_loss(const void* logits, int dtype, int64_t rows, int64_t rows_per_batch,
+                        int64_t batch_stride, int64_t row_stride, int64_t V,
+                        const int64_t* targets, int64_t ignore_index, const void* cu_seqlens,
+                        int cu_is64, int64_t uniform_len, int64_t pairs, const float* ref_logp,
+                        float beta, float label_smoothing, float inv_denominator,
+                        float grad_scale, float* logp, float* stats, float* coef, float* margins,
+                        float* loss, void* dlogits, void* stream) {
+  MHC_TRY_BEGIN
+  const LogitsArg l = {logits, dtype, rows, rows_per_batch, batch_stride, row_stride, V, targets, ignore_index};
+  MHC_CHK(check_logits(__func__, l));
+  MHC_REQ(pairs >= 1 && pairs < ((int64_t)1 << 30), "%s: pairs=%lld must be in [1, 2^30)", __func__, (long long)pairs);
+  MHC_REQ(cu_seqlens || (uniform_len >= 0 && uniform_len <= rows), "%s: uniform_len=%lld must be in [0, rows]", __func__, (long long)uniform_len);
+  MHC_REQ(label_smoothing >= 0.f && label_smoothing < 1.f, "%s: label_smoothing must be in [0, 1)", __func__);
+  MHC_REQ(margins && loss && (rows == 0 || (ref_logp && logp && stats && coef)), "%s: NULL pointer", __func__);
+  MHC_REQ(aligned16(stats), "%s: stats must be 16-byte aligned", __func__);
+  const PreferenceArg a = {cu_seqlens, cu_is64, uniform_len, pairs, ref_logp, beta, label_smoothing, inv_denominator, grad_scale};
+  const PreferenceOut o = {logp, stats, coef, margins, loss, dlogits};
+  return launch_preference(l, a, o, as_stream(stream));
+  MHC_TRY_END
+}
+
+// Workspace of the policy loss: a counter and 1 / D, then two fp64 sums for
+// each cluster of blocks (at most 8 blocks of 128 threads an SM).
+static constexpr size_t kLossHeader = 256;
+size_t mhc_policy_workspace_bytes(void) {
+  return kLossHeader + (size_t)sm_count() * 8 * 2 * sizeof(double);
+}
+
+int mhc_policy_loss(const void* logits, int dtype, int64_t rows, int64_t rows_per_batch,
+                    int64_t batch_stride, int64_t row_stride, int64_t V, const int64_t* targets,
+                    int64_t ignore_index, const float* old_logp, const float* advantages,
+                    const float* ref_logp, float clip_low, float clip_high, float kl_coef,
+                    float inv_denominator, float grad_scale, float* logp, float* stats,
+                    float* coef, float* loss, float* kl, void* dlogits, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  MHC_TRY_BEGIN
+  const LogitsArg l = {logits, dtype, rows, rows_per_batch, batch_stride, row_stride, V, targets, ignore_index};
+  MHC_CHK(check_logits(__func__, l));
+  MHC_REQ(clip_low >= 0.f && clip_high >= 0.f, "%s: clip_low and clip_high must be >= 0", __func__);
+  MHC_REQ(kl_coef == 0.f || ref_logp, "%s: kl_coef needs ref_logp", __func__);
+  MHC_REQ(inv_denominator >= 0.f, "%s: inv_denominator must be >= 0", __func__);
+  MHC_REQ(loss && kl && (rows == 0 || (old_logp && advantages && logp && stats && coef)), "%s: NULL pointer", __func__);
+  if (!workspace || workspace_bytes < mhc_policy_workspace_bytes())
+    return set_error(MHC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", __func__, workspace_bytes, mhc_policy_workspace_bytes());
+  MHC_REQ(aligned16(stats) && aligned16(workspace), "%s: stats and workspace must be 16-byte aligned", __func__);
+  const PolicyArg a = {old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, inv_denominator, grad_scale};
+  char* ws = static_cast<char*>(workspace);
+  const PolicyOut o = {logp, stats, coef, loss, kl, reinterpret_cast<unsigned*>(ws),
+                       reinterpret_cast<float*>(ws) + 1, reinterpret_cast<double*>(ws + kLossHeader), dlogits};
+  return launch_policy(l, a, o, as_stream(stream));
+  MHC_TRY_END
+}
+
 }  // extern "C"

@@ -192,4 +192,44 @@ int launch_qlinear_bwd_dx(const void* dy, int dydt, const uint32_t* wq, const vo
                           const void* biases, int sdt, void* dx, int64_t M, int N, int K,
                           int group_size, int bits, cudaStream_t st);
 
+// ---- losses on logits (mhc_loss.cu) -------------------------------------------
+// Row t of the logits: logits + (t / per_batch) batch_stride + (t % per_batch)
+// row_stride (elements), vocab contiguous values.
+struct LogitsArg {
+  const void* logits;
+  int dtype;
+  int64_t rows, per_batch, batch_stride, row_stride, vocab;
+  const int64_t* targets;
+  int64_t ignore;
+};
+struct PreferenceArg {
+  const void* cu_seqlens;  // null: `uniform` rows a sequence
+  int cu_is64;
+  int64_t uniform, pairs;
+  const float* ref;
+  float beta, smoothing, inv_d, grad_scale;
+};
+struct PreferenceOut {
+  float *logp, *stats, *coef, *margins, *loss;
+  void* dlogits;  // null: no gradient
+};
+struct PolicyArg {
+  const float *old, *adv, *ref;  // ref null: no KL term
+  float clip_low, clip_high, kl_coef, inv_d, grad_scale;  // inv_d 0: 1 / valid tokens
+};
+struct PolicyOut {
+  float *logp, *stats, *coef, *loss, *kl;
+  // workspace: a counter, 1 / D, and two sums a cluster of blocks
+  unsigned* ticket;
+  float* inv_d;
+  double* partial;
+  void* dlogits;  // null: no gradient
+};
+int launch_token_logprobs(const LogitsArg& l, float* logp, float* stats, cudaStream_t st);
+int launch_logits_grad(const LogitsArg& l, const float* stats, const float* coef, float scale,
+                       const float* scale_ptr, int unless_one, void* dlogits, cudaStream_t st);
+int launch_preference(const LogitsArg& l, const PreferenceArg& a, const PreferenceOut& o,
+                      cudaStream_t st);
+int launch_policy(const LogitsArg& l, const PolicyArg& a, const PolicyOut& o, cudaStream_t st);
+
 }  // namespace mhc

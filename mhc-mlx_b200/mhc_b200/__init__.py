@@ -8,6 +8,8 @@ mhc_b200.metal under the reference's names.
 
 from .diagnostics import diagnostics
 from .layer import MHCLayer, MHCRewire
+from .losses import (policy_loss, policy_loss_grad, preference_loss, preference_loss_grad,
+                     token_logprobs)
 from .patching import AutoPatcher
 from .quantized import QuantizedLinear
 from .utils import residual_add_agg
@@ -15,4 +17,5 @@ from .utils import residual_add_agg
 __version__ = "1.0.0"
 
 __all__ = ["MHCLayer", "MHCRewire", "diagnostics", "residual_add_agg", "AutoPatcher",
-           "QuantizedLinear", "__version__"]
+           "QuantizedLinear", "token_logprobs", "preference_loss", "preference_loss_grad",
+           "policy_loss", "policy_loss_grad", "__version__"]

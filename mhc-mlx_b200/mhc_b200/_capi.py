@@ -22,6 +22,8 @@ MHC_F32, MHC_F16, MHC_BF16 = 0, 1, 2
 MHC_OK, MHC_ERR_INVALID, MHC_ERR_CUDA, MHC_ERR_UNSUPPORTED, MHC_ERR_WORKSPACE = 0, 1, 2, 3, 4
 
 _P = c_void_p
+# logits, dtype, rows, rows_per_batch, batch_stride, row_stride, V, targets, ignore_index
+_LOGITS = (_P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, _P, c_int64)
 # name -> (restype, argtypes); mirrors include/mhc_b200.h
 SIGNATURES: dict[str, tuple] = {
     "mhc_last_error": (ctypes.c_char_p, []),
@@ -75,6 +77,13 @@ SIGNATURES: dict[str, tuple] = {
                                      _P]),
     "mhc_residual_add_agg_bwd": (c_int, [_P, c_int, _P, c_int, _P, _P, _P, c_int, _P, c_int64,
                                          c_int, c_int, _P, c_size_t, _P]),
+    "mhc_token_logprobs": (c_int, [*_LOGITS, _P, _P, _P]),
+    "mhc_logits_grad": (c_int, [*_LOGITS, _P, _P, c_float, _P, c_int, _P, _P]),
+    "mhc_preference_loss": (c_int, [*_LOGITS, _P, c_int, c_int64, c_int64, _P, c_float, c_float,
+                                    c_float, c_float, _P, _P, _P, _P, _P, _P, _P]),
+    "mhc_policy_workspace_bytes": (c_size_t, []),
+    "mhc_policy_loss": (c_int, [*_LOGITS, _P, _P, _P, c_float, c_float, c_float, c_float, c_float,
+                                _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
 }
 
 _lib = None
