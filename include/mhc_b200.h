@@ -397,6 +397,67 @@ MHC_API int mhc_policy_loss(const void* logits, int dtype, int64_t rows, int64_t
                             float* loss, float* kl, void* dlogits, void* workspace,
                             size_t workspace_bytes, void* stream);
 
+/* ---- AdamW over many tensors --------------------------------------------------
+ * No counterpart in the reference.  One launch (one per 1000 tensors) updates
+ * `count` parameters of one type in place:
+ *   m = beta1 m + one_minus_beta1 g,  v = beta2 v + one_minus_beta2 g^2
+ *   p = decay p - step_size m / (sqrt(v) inv_sqrt_correction + eps)
+ * with decay = 1 - lr weight_decay, step_size = lr / (1 - beta1^t),
+ * inv_sqrt_correction = 1 / sqrt(1 - beta2^t); g is the gradient, times
+ * *grad_scale when that device scalar is given.
+ * params, grads (device addresses, contiguous values in the same order), numel
+ * and offsets are HOST arrays, read during the call.  offsets[i], a multiple of
+ * 256, is where tensor i's part of the state begins; parts are padded to a
+ * multiple of 256 elements (the padding starts at 0 and stays so).
+ * state_bits 32: exp_avg (m) and exp_avg_sq (v) are fp32, the scales NULL.
+ * state_bits 8: they hold e4m3 codes of m and of sqrt(v) in units of
+ * exp_avg_scale[e / 256] / exp_avg_sq_scale[e / 256], powers of two; rounding is
+ * up or down by a hash of the element's place in the state and `key`.  The
+ * moments of a non-finite gradient become NaN and stay so.
+ * master (nullable, 16-bit parameters): fp32 weights that the update is made
+ * on; the parameter receives their rounded values.
+ * State buffers and master are 16-byte aligned. */
+MHC_API int mhc_adamw_step(int count, void* const* params, const void* const* grads,
+                           const int64_t* numel, const int64_t* offsets, int dtype,
+                           int state_bits, void* exp_avg, float* exp_avg_scale,
+                           void* exp_avg_sq, float* exp_avg_sq_scale, float* master,
+                           float beta1, float one_minus_beta1, float beta2,
+                           float one_minus_beta2, float decay, float step_size,
+                           float inv_sqrt_correction, float eps, const float* grad_scale,
+                           uint32_t key, void* stream);
+
+/* ---- linear layer with its epilogue, and its gradients ------------------------
+ * No counterpart in the reference: the projections that MHCRewire wraps, in
+ * bf16 or fp16 (one type for all operands), fp32 accumulation.
+ *   z = x W^T + bias,  y = act(z) + residual
+ *   dz = dy act'(z),  dx = dz W,  dw = dz^T x,  dbias = sum over rows of dz
+ * x [M, K], w [N, K], y / residual / dy [M, N], bias / dbias [N]; values along a
+ * row are contiguous, ld* is the distance between rows in elements.  act: 0 none,
+ * 1 relu, 2 silu, 3 gelu (erf).  bias and residual may be NULL.
+ * z (nullable in the forward; NULL in the backward for act 0) holds the
+ * pre-activation rounded to the type, 16-byte aligned, ldz >= N a multiple of 8.
+ * dx, dw and dbias may each be NULL.  dz is rounded to the type before its
+ * products.  Rows that do not begin on 16-byte boundaries are copied to padded
+ * ones in the workspace.  1 <= N, K < 2^31; 0 <= M < 2^31 (M = 0 writes zeros
+ * into dw and dbias).  Workspace: the matching *_workspace_bytes() for the same
+ * pointers. */
+MHC_API size_t mhc_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w,
+                                              int64_t ldw, int64_t M, int64_t N, int64_t K);
+MHC_API int mhc_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                           const void* bias, const void* residual, int64_t ldr, int dtype,
+                           int act, void* z, int64_t ldz, void* y, int64_t ldy, int64_t M,
+                           int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                           void* stream);
+MHC_API size_t mhc_linear_bwd_workspace_bytes(const void* dy, int64_t ldy, const void* x,
+                                              int64_t ldx, const void* w, int64_t ldw, int act,
+                                              int want_dx, int want_dw, int want_dbias,
+                                              int64_t M, int64_t N, int64_t K);
+MHC_API int mhc_linear_bwd(const void* dy, int64_t ldy, const void* z, int64_t ldz,
+                           const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
+                           int act, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                           void* dbias, int64_t M, int64_t N, int64_t K, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -611,4 +611,130 @@ int mhc_policy_loss(const void* logits, int dtype, int64_t rows, int64_t rows_pe
   MHC_TRY_END
 }
 
+// ---- AdamW ----
+int mhc_adamw_step(int count, void* const* params, const void* const* grads, const int64_t* numel,
+                   const int64_t* offsets, int dtype, int state_bits, void* exp_avg,
+                   float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale, float* master,
+                   float beta1, float one_minus_beta1, float beta2, float one_minus_beta2,
+                   float decay, float step_size, float inv_sqrt_correction, float eps,
+                   const float* grad_scale, uint32_t key, void* stream) {
+  MHC_TRY_BEGIN
+  MHC_CHK(check_dtype(__func__, "params", dtype));
+  MHC_REQ(count >= 0, "%s: count=%d must be >= 0", __func__, count);
+  MHC_REQ(state_bits == 8 || state_bits == 32, "%s: state_bits=%d must be 8 or 32", __func__, state_bits);
+  MHC_REQ(!master || dtype != MHC_F32, "%s: master weights are for 16-bit parameters", __func__);
+  if (count == 0) return MHC_OK;
+  MHC_REQ(params && grads && numel && offsets, "%s: NULL array", __func__);
+  MHC_REQ(exp_avg && exp_avg_sq, "%s: NULL state", __func__);
+  MHC_REQ(state_bits == 32 || (exp_avg_scale && exp_avg_sq_scale), "%s: 8-bit state needs its scales", __func__);
+  MHC_REQ(aligned16(exp_avg) && aligned16(exp_avg_sq) && aligned16(master), "%s: the state must be 16-byte aligned", __func__);
+  const uintptr_t size = (uintptr_t)dtype_size(dtype);
+  for (int i = 0; i < count; ++i) {
+    MHC_REQ(numel[i] >= 0, "%s: numel[%d] is negative", __func__, i);
+    MHC_REQ(offsets[i] >= 0 && offsets[i] % 256 == 0 && offsets[i] / 256 < ((int64_t)1 << 32), "%s: offsets[%d] must be a multiple of 256 below 2^40", __func__, i);
+    MHC_REQ(numel[i] == 0 || (params[i] && grads[i]), "%s: NULL tensor %d", __func__, i);
+    MHC_REQ(reinterpret_cast<uintptr_t>(params[i]) % size == 0 && reinterpret_cast<uintptr_t>(grads[i]) % size == 0, "%s: tensor %d is not aligned to its type", __func__, i);
+  }
+  const AdamWArg a = {count, params, grads, numel, offsets, dtype, state_bits, exp_avg, exp_avg_sq,
+                      exp_avg_scale, exp_avg_sq_scale, master, beta1, one_minus_beta1, beta2,
+                      one_minus_beta2, decay, step_size, inv_sqrt_correction, eps, grad_scale, key};
+  return launch_adamw(a, as_stream(stream));
+  MHC_TRY_END
+}
+
+// ---- linear layer with its epilogue ----
+static int check_linear(const char* fn, int dtype, int act, int64_t M, int64_t N, int64_t K) {
+  if (dtype != MHC_BF16 && dtype != MHC_F16)
+    return set_error(dtype_ok(dtype) ? MHC_ERR_UNSUPPORTED : MHC_ERR_INVALID, "%s: dtype %d is not MHC_F16 or MHC_BF16", fn, dtype);
+  MHC_REQ(act >= 0 && act <= 3, "%s: act=%d must be in [0, 3]", fn, act);
+  MHC_REQ(M >= 0 && M < ((int64_t)1 << 31), "%s: M=%lld must be in [0, 2^31)", fn, (long long)M);
+  MHC_REQ(N >= 1 && N < ((int64_t)1 << 31), "%s: N=%lld must be in [1, 2^31)", fn, (long long)N);
+  MHC_REQ(K >= 1 && K < ((int64_t)1 << 31), "%s: K=%lld must be in [1, 2^31)", fn, (long long)K);
+  return MHC_OK;
+}
+static int check_rows(const char* fn, const char* what, const void* p, int64_t ld, int64_t cols) {
+  MHC_REQ(p, "%s: NULL %s", fn, what);
+  MHC_REQ(reinterpret_cast<uintptr_t>(p) % 2 == 0, "%s: %s is not aligned to its type", fn, what);
+  MHC_REQ(ld >= cols, "%s: rows of %s are %lld apart, %lld values long", fn, what, (long long)ld, (long long)cols);
+  return MHC_OK;
+}
+
+size_t mhc_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                      int64_t M, int64_t N, int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  return linear_fwd_ws_bytes(x, ldx, w, ldw, M, N, K);
+}
+
+int mhc_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                   const void* residual, int64_t ldr, int dtype, int act, void* z, int64_t ldz,
+                   void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  MHC_TRY_BEGIN
+  MHC_CHK(check_linear(__func__, dtype, act, M, N, K));
+  if (M == 0) return MHC_OK;
+  MHC_CHK(check_rows(__func__, "x", x, ldx, K));
+  MHC_CHK(check_rows(__func__, "w", w, ldw, K));
+  MHC_CHK(check_rows(__func__, "y", y, ldy, N));
+  if (bias) MHC_CHK(check_rows(__func__, "bias", bias, N, N));
+  if (residual) MHC_CHK(check_rows(__func__, "residual", residual, ldr, N));
+  if (z) {
+    MHC_CHK(check_rows(__func__, "z", z, ldz, N));
+    MHC_REQ(aligned16(z) && ldz % 8 == 0, "%s: z must be 16-byte aligned, its rows multiples of 8", __func__);
+  }
+  const LinearArg l = {x, w, bias, residual, ldx, ldw, ldr, dtype, act, M, N, K, z, ldz, y, ldy, workspace, workspace ? workspace_bytes : 0};
+  if (l.workspace_bytes < linear_fwd_ws_bytes(x, ldx, w, ldw, M, N, K))
+    return set_error(MHC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", __func__, l.workspace_bytes, linear_fwd_ws_bytes(x, ldx, w, ldw, M, N, K));
+  MHC_REQ(aligned16(workspace), "%s: the workspace must be 16-byte aligned", __func__);
+  return launch_linear_fwd(l, as_stream(stream));
+  MHC_TRY_END
+}
+
+size_t mhc_linear_bwd_workspace_bytes(const void* dy, int64_t ldy, const void* x, int64_t ldx,
+                                      const void* w, int64_t ldw, int act, int want_dx,
+                                      int want_dw, int want_dbias, int64_t M, int64_t N,
+                                      int64_t K) {
+  if (M < 1 || N < 1 || K < 1) return 0;
+  char some = 0;  // stands for an output that is wanted
+  LinearGradArg l = {};
+  l.dy = dy; l.ldy = ldy; l.x = x; l.ldx = ldx; l.w = w; l.ldw = ldw; l.act = act;
+  l.M = M; l.N = N; l.K = K;
+  l.dx = want_dx ? &some : nullptr;
+  l.dw = want_dw ? &some : nullptr;
+  l.dbias = want_dbias ? &some : nullptr;
+  return linear_bwd_ws_bytes(l);
+}
+
+int mhc_linear_bwd(const void* dy, int64_t ldy, const void* z, int64_t ldz, const void* x,
+                   int64_t ldx, const void* w, int64_t ldw, int dtype, int act, void* dx,
+                   int64_t lddx, void* dw, int64_t lddw, void* dbias, int64_t M, int64_t N,
+                   int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+  MHC_TRY_BEGIN
+  MHC_CHK(check_linear(__func__, dtype, act, M, N, K));
+  if (dw) MHC_CHK(check_rows(__func__, "dw", dw, lddw, K));
+  if (M == 0) {
+    cudaError_t e = cudaSuccess;
+    if (dw) e = cudaMemset2DAsync(dw, (size_t)lddw * 2, 0, (size_t)K * 2, (size_t)N, as_stream(stream));
+    if (dbias && e == cudaSuccess) e = cudaMemsetAsync(dbias, 0, (size_t)N * 2, as_stream(stream));
+    if (e != cudaSuccess) return set_error(MHC_ERR_CUDA, "%s: %s", __func__, cudaGetErrorString(e));
+    return MHC_OK;
+  }
+  MHC_CHK(check_rows(__func__, "dy", dy, ldy, N));
+  if (act != 0) {
+    MHC_CHK(check_rows(__func__, "z", z, ldz, N));
+    MHC_REQ(aligned16(z) && ldz % 8 == 0, "%s: z must be 16-byte aligned, its rows multiples of 8", __func__);
+  }
+  if (dx) {
+    MHC_CHK(check_rows(__func__, "dx", dx, lddx, K));
+    MHC_CHK(check_rows(__func__, "w", w, ldw, K));
+  }
+  if (dw) MHC_CHK(check_rows(__func__, "x", x, ldx, K));
+  if (dbias) MHC_CHK(check_rows(__func__, "dbias", dbias, N, N));
+  const LinearGradArg l = {dy, z, x, w, ldy, ldz, ldx, ldw, dtype, act, M, N, K, dx, dw, dbias, lddx, lddw, workspace, workspace ? workspace_bytes : 0};
+  if (l.workspace_bytes < linear_bwd_ws_bytes(l))
+    return set_error(MHC_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", __func__, l.workspace_bytes, linear_bwd_ws_bytes(l));
+  MHC_REQ(aligned16(workspace), "%s: the workspace must be 16-byte aligned", __func__);
+  return launch_linear_bwd(l, as_stream(stream));
+  MHC_TRY_END
+}
+
 }  // extern "C"

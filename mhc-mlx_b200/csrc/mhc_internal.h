@@ -232,4 +232,50 @@ int launch_preference(const LogitsArg& l, const PreferenceArg& a, const Preferen
                       cudaStream_t st);
 int launch_policy(const LogitsArg& l, const PolicyArg& a, const PolicyOut& o, cudaStream_t st);
 
+// ---- AdamW over many tensors (mhc_adamw.cu) -----------------------------------
+struct AdamWArg {
+  int count;  // host arrays of this length
+  void* const* params;
+  const void* const* grads;
+  const int64_t* numel;
+  const int64_t* offsets;  // into the state, multiples of 256
+  int dtype, state_bits;
+  void *exp_avg, *exp_avg_sq;  // fp32, or e4m3 codes of m and sqrt(v)
+  float *exp_avg_scale, *exp_avg_sq_scale, *master;
+  float beta1, one_minus_beta1, beta2, one_minus_beta2, decay, step_size, inv_sqrt_correction, eps;
+  const float* grad_scale;
+  uint32_t key;
+};
+int launch_adamw(const AdamWArg& a, cudaStream_t st);
+
+// ---- linear layer with its epilogue (mhc_linear.cu) ---------------------------
+// act: 0 none, 1 relu, 2 silu, 3 gelu (erf).  Leading dimensions in elements.
+struct LinearArg {
+  const void *x, *w, *bias, *residual;  // bias, residual nullable
+  int64_t ldx, ldw, ldr;
+  int dtype, act;
+  int64_t M, N, K;
+  void* z;  // nullable: the pre-activation, rows padded to a multiple of 8
+  int64_t ldz;
+  void* y;
+  int64_t ldy;
+  void* workspace;
+  size_t workspace_bytes;
+};
+struct LinearGradArg {
+  const void *dy, *z, *x, *w;  // z null without activation
+  int64_t ldy, ldz, ldx, ldw;
+  int dtype, act;
+  int64_t M, N, K;
+  void *dx, *dw, *dbias;  // each nullable
+  int64_t lddx, lddw;
+  void* workspace;
+  size_t workspace_bytes;
+};
+size_t linear_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
+                           int64_t N, int64_t K);
+size_t linear_bwd_ws_bytes(const LinearGradArg& l);
+int launch_linear_fwd(const LinearArg& l, cudaStream_t st);
+int launch_linear_bwd(const LinearGradArg& l, cudaStream_t st);
+
 }  // namespace mhc

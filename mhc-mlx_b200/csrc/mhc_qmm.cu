@@ -32,99 +32,16 @@
 // Every wait is bounded: a barrier that never completes makes the CTA write
 // NaN into its output tile and return (after waiting, again bounded, for its
 // own copies and MMAs), so a fault shows as NaN instead of a hang.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
 #include <cstdlib>
-#include <mutex>
 
-#include "mhc_common.cuh"
 #include "mhc_internal.h"
+#include "mhc_tcgen05.cuh"
 
 namespace mhc {
 namespace {
 
 constexpr int kBM = 128, kBK = 64, kGroup = 64;
 constexpr int kThreads = 320, kDqThreads = 256;
-constexpr unsigned kWaitLimit = 1u << 22;
-
-// Shared-memory descriptor of a 128-byte-swizzled operand tile (tcgen05
-// matrix descriptor): start address, leading / stride byte offsets (in 16-byte
-// units), version 1, layout SWIZZLE_128B.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFFu) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFFu) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
-// Instruction descriptor, kind::f16: fp32 accumulate, A and B of one 16-bit
-// type (bf16: 1, fp16: 0), A K-major, B K- or MN-major, M = 128, N = BN.
-__host__ __device__ constexpr uint32_t f16_idesc(uint32_t ab, uint32_t b_mn, int M, int N) {
-  return (1u << 4) | (ab << 7) | (ab << 10) | (b_mn << 16) | ((uint32_t)(N >> 3) << 17) |
-         ((uint32_t)(M >> 4) << 24);
-}
-
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y,
-                                       uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];\n" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
-                                         uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
-          smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-}
-
-// 32 consecutive accumulator columns of this thread's row (TMEM lane).
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, "
-      "%28, %29, %30, %31}, [%32];\n"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-}
-
-// Bounded barrier wait that also gives up once another role has aborted.
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, unsigned parity,
-                                              volatile int* abort_flag) {
-  for (unsigned k = 0; k < kWaitLimit; ++k) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((k & 1023u) == 1023u && *abort_flag) return false;
-  }
-  return false;
-}
 
 // Packed pairs of 16-bit floats (the dequantisation runs two values per
 // instruction in the scales' dtype ST, then converts to the operand dtype XT).
@@ -714,38 +631,6 @@ __global__ void k_transpose_pack4(const uint32_t* __restrict__ w, uint32_t* __re
 }
 
 // ------------------------------------------------------------------ host --
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, []() {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    else
-      (void)cudaGetLastError();
-  });
-  return fn;
-}
-
-int make_map(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner,
-             uint64_t outer, uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer,
-             CUtensorMapSwizzle sw) {
-  auto fn = encode_fn();
-  if (!fn) return set_error(MHC_ERR_CUDA, "qlinear: cuTensorMapEncodeTiled is unavailable");
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {row_bytes};
-  const cuuint32_t box[2] = {box_inner, box_outer};
-  const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(MHC_ERR_CUDA, "qlinear: tensor map encode failed (%d)", (int)r);
-  return MHC_OK;
-}
-
 template <int BN, bool BWD, typename XT, typename ST>
 int run_qlinear(const void* a, const uint32_t* wq, const void* scales, const void* biases,
                 const void* bias, void* out, int64_t M, int N, int K, cudaStream_t st) {
@@ -753,15 +638,15 @@ int run_qlinear(const void* a, const uint32_t* wq, const void* scales, const voi
   const CUtensorMapDataType adt =
       std::is_same<XT, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int RED = BWD ? N : K;
-  int r = make_map(&ma, adt, a, (uint64_t)RED, (uint64_t)M, (uint64_t)RED * 2, kBK, kBM,
+  int r = make_tensor_map("qlinear", &ma, adt, a, (uint64_t)RED, (uint64_t)M, (uint64_t)RED * 2, kBK, kBM,
                    CU_TENSOR_MAP_SWIZZLE_128B);
   if (r != MHC_OK) return r;
   // packed words: [N rows][K / 8 words]
   if constexpr (BWD)
-    r = make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wq, (uint64_t)K / 8, (uint64_t)N,
+    r = make_tensor_map("qlinear", &mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wq, (uint64_t)K / 8, (uint64_t)N,
                  (uint64_t)K / 2, BN / 8, kBK, CU_TENSOR_MAP_SWIZZLE_NONE);
   else
-    r = make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wq, (uint64_t)K / 8, (uint64_t)N,
+    r = make_tensor_map("qlinear", &mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wq, (uint64_t)K / 8, (uint64_t)N,
                  (uint64_t)K / 2, kBK / 8, BN, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (r != MHC_OK) return r;
   auto kern = k_qlinear<BN, BWD, XT, ST>;
@@ -782,10 +667,10 @@ int run_qlinear_fwd_tm(const void* x, const uint32_t* wq, const void* scales, co
   CUtensorMap mx, mw;
   const CUtensorMapDataType xdt =
       std::is_same<XT, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  int r = make_map(&mx, xdt, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, kBK, kTmTok,
+  int r = make_tensor_map("qlinear", &mx, xdt, x, (uint64_t)K, (uint64_t)M, (uint64_t)K * 2, kBK, kTmTok,
                    CU_TENSOR_MAP_SWIZZLE_128B);
   if (r != MHC_OK) return r;
-  r = make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wq, (uint64_t)K / 8, (uint64_t)N,
+  r = make_tensor_map("qlinear", &mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wq, (uint64_t)K / 8, (uint64_t)N,
                (uint64_t)K / 2, 4, kTmFeat, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (r != MHC_OK) return r;
   auto kern = k_qlinear_tm<false, XT, ST>;
@@ -806,18 +691,18 @@ int run_qlinear_bwd_tm(const void* dy, const uint32_t* wt, const void* scales_t,
   CUtensorMap md, mw, ms, mb;
   const CUtensorMapDataType xdt =
       std::is_same<XT, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  int r = make_map(&md, xdt, dy, (uint64_t)N, (uint64_t)M, (uint64_t)N * 2, kBK, kTmTok,
+  int r = make_tensor_map("qlinear", &md, xdt, dy, (uint64_t)N, (uint64_t)M, (uint64_t)N * 2, kBK, kTmTok,
                    CU_TENSOR_MAP_SWIZZLE_128B);
   if (r != MHC_OK) return r;
   // codes of W^T: [K rows][N / 8 words]
-  r = make_map(&mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wt, (uint64_t)N / 8, (uint64_t)K,
+  r = make_tensor_map("qlinear", &mw, CU_TENSOR_MAP_DATA_TYPE_INT32, wt, (uint64_t)N / 8, (uint64_t)K,
                (uint64_t)N / 2, 4, kTmFeat, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (r != MHC_OK) return r;
   // scales / biases of W^T: [K / 64][N] in the activations' dtype
-  r = make_map(&ms, xdt, scales_t, (uint64_t)N, (uint64_t)K / kGroup, (uint64_t)N * 2, kBK, 2,
+  r = make_tensor_map("qlinear", &ms, xdt, scales_t, (uint64_t)N, (uint64_t)K / kGroup, (uint64_t)N * 2, kBK, 2,
                CU_TENSOR_MAP_SWIZZLE_NONE);
   if (r != MHC_OK) return r;
-  r = make_map(&mb, xdt, biases_t, (uint64_t)N, (uint64_t)K / kGroup, (uint64_t)N * 2, kBK, 2,
+  r = make_tensor_map("qlinear", &mb, xdt, biases_t, (uint64_t)N, (uint64_t)K / kGroup, (uint64_t)N * 2, kBK, 2,
                CU_TENSOR_MAP_SWIZZLE_NONE);
   if (r != MHC_OK) return r;
   auto kern = k_qlinear_tm<true, XT, XT>;

@@ -84,6 +84,18 @@ SIGNATURES: dict[str, tuple] = {
     "mhc_policy_workspace_bytes": (c_size_t, []),
     "mhc_policy_loss": (c_int, [*_LOGITS, _P, _P, _P, c_float, c_float, c_float, c_float, c_float,
                                 _P, _P, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "mhc_adamw_step": (c_int, [c_int, _P, _P, _P, _P, c_int, c_int, _P, _P, _P, _P, _P, c_float,
+                               c_float, c_float, c_float, c_float, c_float, c_float, c_float, _P,
+                               ctypes.c_uint32, _P]),
+    "mhc_linear_fwd_workspace_bytes": (c_size_t, [_P, c_int64, _P, c_int64, c_int64, c_int64,
+                                                  c_int64]),
+    "mhc_linear_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, _P, c_int64, c_int, c_int, _P, c_int64,
+                               _P, c_int64, c_int64, c_int64, c_int64, _P, c_size_t, _P]),
+    "mhc_linear_bwd_workspace_bytes": (c_size_t, [_P, c_int64, _P, c_int64, _P, c_int64, c_int,
+                                                  c_int, c_int, c_int, c_int64, c_int64, c_int64]),
+    "mhc_linear_bwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int, _P,
+                               c_int64, _P, c_int64, _P, c_int64, c_int64, c_int64, _P, c_size_t,
+                               _P]),
 }
 
 _lib = None

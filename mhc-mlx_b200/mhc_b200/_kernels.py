@@ -563,3 +563,78 @@ def policy_loss(r: LogitRows, old, adv, ref, clip_low: float, clip_high: float, 
               clip_high, kl_coef, inv_d, grad_scale, C.ptr(logp), C.ptr(stats), C.ptr(coef),
               C.ptr(loss), C.ptr(kl), C.ptr(dlogits), C.ptr(ws), nb, C.stream_of(r.logits))
     return loss, logp, kl, dlogits, stats, coef
+
+
+# ------------------------------------------------------------------ AdamW --
+def adamw_step(dev: torch.device, count: int, params, grads, numel, offsets, dtype, bits: int,
+               exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, master, b1, omb1, b2, omb2,
+               decay, step_size, inv_sqrt_correction, eps, grad_scale, key: int) -> None:
+    """params .. offsets: ctypes arrays of `count` addresses and sizes."""
+    C.require_cuda(exp_avg, grad_scale)
+    with _on(dev):
+        scale = None if grad_scale is None else _f32(grad_scale)
+        _call("mhc_adamw_step", exp_avg, count, params, grads, numel, offsets,
+              C.dtype_code(dtype), bits, C.ptr(exp_avg), C.ptr(exp_avg_scale), C.ptr(exp_avg_sq),
+              C.ptr(exp_avg_sq_scale), C.ptr(master), b1, omb1, b2, omb2, decay, step_size,
+              inv_sqrt_correction, eps, C.ptr(scale), key, C.stream_of(exp_avg))
+
+
+# ----------------------------------------------------------------- linear --
+def _rows2d(t: torch.Tensor) -> torch.Tensor:
+    """[..., C] as [rows, C] with contiguous rows, in place where its strides allow."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+    return t.reshape(-1, t.shape[-1])
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Distance between the rows of a 2-D tensor (of one row: its length)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _spread(t: torch.Tensor) -> torch.Tensor:
+    """Rows that overlap (an expanded tensor) cannot be walked: copied."""
+    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
+
+
+def linear_fwd(x, weight, bias, residual, act: int, keep_z: bool):
+    """(y, z): z is the pre-activation, rows padded to a multiple of 8, or None."""
+    dev = C.require_cuda(x, weight, bias, residual)
+    N, Kc = weight.shape
+    with _on(dev):
+        x2, w2 = _spread(_rows2d(x)), _spread(_rows2d(weight))
+        M = x2.shape[0]
+        r2 = None if residual is None else _spread(_rows2d(residual))
+        b1 = None if bias is None else _c(bias)
+        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
+        ldz = (N + 7) // 8 * 8
+        z = torch.empty(M, ldz, dtype=x.dtype, device=dev) if keep_z else None
+        args = (C.ptr(x2), _ld(x2), C.ptr(w2), _ld(w2))
+        nb = int(C.query("mhc_linear_fwd_workspace_bytes", *args, M, N, Kc))
+        ws = _ws(nb, dev) if nb else None
+        _call("mhc_linear_fwd", x2, *args, C.ptr(b1), C.ptr(r2), 0 if r2 is None else _ld(r2),
+              C.dtype_code(x.dtype), act, C.ptr(z), ldz, C.ptr(y), N, M, N, Kc, C.ptr(ws), nb,
+              C.stream_of(x2))
+    return y, z
+
+
+def linear_bwd(dy, z, x, weight, act: int, want_dx: bool, want_dw: bool, want_db: bool):
+    """(dx, dweight, dbias), None where not wanted."""
+    dev = C.require_cuda(dy, x, weight)
+    N, Kc = weight.shape
+    with _on(dev):
+        d2, x2, w2 = _spread(_rows2d(dy)), _spread(_rows2d(x)), _spread(_rows2d(weight))
+        M = x2.shape[0]
+        new = lambda *s: torch.empty(*s, dtype=x.dtype, device=dev)  # noqa: E731
+        dx = new(*x.shape) if want_dx else None
+        dw = new(N, Kc) if want_dw else None
+        db = new(N) if want_db else None
+        args = (C.ptr(d2), _ld(d2))
+        ops = (C.ptr(x2), _ld(x2), C.ptr(w2), _ld(w2))
+        nb = int(C.query("mhc_linear_bwd_workspace_bytes", *args, *ops, act, int(want_dx),
+                         int(want_dw), int(want_db), M, N, Kc))
+        ws = _ws(nb, dev) if nb else None
+        _call("mhc_linear_bwd", x2, *args, C.ptr(z), 0 if z is None else z.shape[1], *ops,
+              C.dtype_code(x.dtype), act, C.ptr(dx), Kc, C.ptr(dw), Kc, C.ptr(db), M, N, Kc,
+              C.ptr(ws), nb, C.stream_of(x2))
+    return dx, dw, db

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -75,3 +77,76 @@ def test_loss_entry_points_check_their_arguments():
         _capi.call("mhc_preference_loss", *rows, 5, None, -100, None, 0, 0, 0, None, 0.1, 0.0, 1.0,
                    1.0, None, None, None, None, None, None, None)
     assert _capi.query("mhc_policy_workspace_bytes") >= 256 + 16 * 148
+
+
+def test_adamw_refusals():
+    p = torch.nn.Parameter(torch.zeros(4, 4))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mhc_b200.AdamW([p])
+    for kw, match in [(dict(state_bits=16), "state_bits"), (dict(lr=-1.0), "lr"),
+                      (dict(lr=torch.tensor(0.1)), "lr"), (dict(betas=(1.0, 0.9)), "betas"),
+                      (dict(eps=-1.0), "eps"), (dict(weight_decay=-0.1), "weight_decay")]:
+        with pytest.raises(ValueError, match=match):
+            mhc_b200.AdamW([p], **kw)
+    with pytest.raises(ValueError, match="dtype"):
+        mhc_b200.AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float64))])
+    with pytest.raises(ValueError, match="dense"):
+        mhc_b200.AdamW([torch.zeros(4, 8)[:, ::2].requires_grad_(True)])
+
+
+def test_adamw_entry_point_checks_its_arguments():
+    tail = (0.9, 0.1, 0.9, 0.1, 1.0, 0.1, 1.0, 1e-8, None, 0, None)
+    none = (None, None, None, None)
+    with pytest.raises(ValueError, match="state_bits"):
+        _capi.call("mhc_adamw_step", 0, *none, 0, 4, None, None, None, None, None, *tail)
+    with pytest.raises(ValueError, match="master"):
+        _capi.call("mhc_adamw_step", 0, *none, 0, 32, None, None, None, None, 256, *tail)
+    with pytest.raises(ValueError, match="NULL"):
+        _capi.call("mhc_adamw_step", 1, *none, 0, 32, None, None, None, None, None, *tail)
+    one = (ctypes.c_uint64 * 1)(256)
+    size, off = (ctypes.c_int64 * 1)(4), (ctypes.c_int64 * 1)(100)
+    with pytest.raises(ValueError, match="multiple of 256"):
+        _capi.call("mhc_adamw_step", 1, one, one, size, off, 0, 32, 256, None, 256, None, None, *tail)
+    with pytest.raises(ValueError, match="scales"):
+        _capi.call("mhc_adamw_step", 1, one, one, size, off, 0, 8, 256, None, 256, None, None, *tail)
+    _capi.call("mhc_adamw_step", 0, *none, 0, 32, None, None, None, None, None, *tail)
+
+
+def test_linear_refusals():
+    x, w = torch.zeros(3, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.bfloat16)
+    b, r = torch.zeros(4, dtype=torch.bfloat16), torch.zeros(3, 4, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mhc_b200.linear_act(x, w, b, residual=r)
+    for args, kw, match in [((x.float(), w.float()), {}, "float16 or bfloat16"),
+                            ((x, w.half()), {}, "weight"), ((x, w[0]), {}, "weight"),
+                            ((x, w[:0]), {}, "weight"), ((x[:, :7], w), {}, "x must"),
+                            ((x, w, b[:3]), {}, "bias"), ((x, w, b.float()), {}, "bias"),
+                            ((x, w), dict(residual=r[:2]), "residual"),
+                            ((x, w), dict(residual=r.half()), "residual"),
+                            ((x, w), dict(activation="tanh"), "activation")]:
+        with pytest.raises(ValueError, match=match):
+            mhc_b200.linear_act(*args, **kw)
+    with pytest.raises(ValueError, match="activation"):
+        mhc_b200.FusedLinear(8, 4, activation="swish")
+
+
+def test_linear_entry_points_check_their_arguments():
+    fwd = lambda x=256, ldx=8, dt=2, act=0, M=1, N=4, K=8: _capi.call(  # noqa: E731
+        "mhc_linear_fwd", x, ldx, 256, 8, None, None, 0, dt, act, None, 0, 256, 4, M, N, K, None, 0,
+        None)
+    with pytest.raises(_capi.MHCError, match="dtype"):
+        fwd(dt=0)
+    for kw, match in [(dict(dt=9), "dtype"), (dict(act=4), "act"), (dict(M=-1), "M="),
+                      (dict(N=0), "N="), (dict(K=0), "K="), (dict(x=None), "NULL x"),
+                      (dict(x=257), "aligned"), (dict(ldx=7), "apart")]:
+        with pytest.raises(ValueError, match=match):
+            fwd(**kw)
+    with pytest.raises(_capi.MHCError, match="workspace"):
+        fwd(x=258, M=100)  # rows that have to be padded
+    fwd(M=0)
+    query = lambda *a: _capi.query("mhc_linear_bwd_workspace_bytes", *a)  # noqa: E731
+    assert query(256, 64, 256, 64, 256, 64, 0, 1, 1, 0, 100, 64, 64) == 0
+    assert query(256, 64, 256, 64, 256, 64, 2, 1, 0, 0, 100, 64, 64) >= 100 * 64 * 2
+    with pytest.raises(ValueError, match="z"):
+        _capi.call("mhc_linear_bwd", 256, 64, None, 0, 256, 64, 256, 64, 2, 1, 256, 64, None, 0, None,
+                   100, 64, 64, None, 0, None)
