@@ -15,8 +15,13 @@
 //   warp 0      TMA: slices of 64 along the reduction, 128-byte swizzled, into a
 //               ring that fills shared memory;
 //   warp 1      four MMAs of 128 x BN x 16 a slice into one of two accumulators;
-//   warps 2-9   read the other accumulator back, apply the epilogue and store,
-//               while the next tile's products run.
+//   warps 2-9   read the other accumulator back and apply the epilogue while the
+//               next tile's products run.  A thread holds a row of the tile;
+//               32 rows x 64 columns at a time go through 4 KB of shared memory
+//               of the warp's own, and from there as one TMA store (or, where
+//               the output's rows are not on 16-byte boundaries, row by row with
+//               the lanes along it): stores straight from registers touch 32
+//               rows an instruction.
 // Every wait is bounded: on one that runs out the CTA writes NaN into its
 // remaining tiles and returns.
 //
@@ -62,7 +67,8 @@ template <int BN>
 struct Ring {
   static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
   static constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  static constexpr int kBytes = kStages * kStage + 1024;  // + alignment slack
+  static constexpr int kOut = 8 * 4096;  // the epilogue warps' stages
+  static constexpr int kBytes = kStages * kStage + kOut + 1024;  // + alignment slack
   static_assert(kBytes <= 226 * 1024, "shared memory");
 };
 
@@ -74,7 +80,7 @@ struct Epilogue {
   T* d;               // [M][ldd]
   int64_t ldr, ldz, ldd;
   int M, N;
-  int wide_bias, wide_res, wide_d, wide_z;  // 16-byte accesses are possible
+  int wide_bias, wide_res, wide_d;  // 16-byte accesses are possible
 };
 
 // Up to 8 consecutive values from p as fp32, 0 past n.
@@ -87,15 +93,60 @@ __device__ __forceinline__ void read8(const T* p, bool wide, int n, float (&o)[8
     for (int k = 0; k < 8; ++k) o[k] = k < n ? to_f(p[k]) : 0.f;
   }
 }
+// Eight fp32 values rounded to T.
 template <typename T>
-__device__ __forceinline__ void write8(T* p, bool wide, int n, const float (&v)[8]) {
-  if (wide && n >= 8) {
-    store_vec<T, 8, false>(p, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) p[k] = from_f<T>(v[k]);
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2_16<T>(v[0], v[1]), pack2_16<T>(v[2], v[3]), pack2_16<T>(v[4], v[5]),
+                    pack2_16<T>(v[6], v[7]));
+}
+// A warp's stage: 32 rows of 64 values, 128 bytes a row, 16-byte chunks swizzled
+// by the row as TMA does it.
+__device__ __forceinline__ uint4* chunk_of(uint8_t* stage, int row, int chunk) {
+  return reinterpret_cast<uint4*>(stage + row * 128 + ((chunk ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ uint32_t* pair_of(uint8_t* stage, int row, int pair) {
+  return reinterpret_cast<uint32_t*>(stage + row * 128 + (((pair >> 2) ^ (row & 7)) << 4) + (pair & 3) * 4);
+}
+// Rows of a matrix <-> the stage, lanes along the row: two values a lane.
+template <typename T>
+__device__ __forceinline__ void rows_out(T* p, int64_t ld, uint8_t* stage, int lane, int rows, int cols) {
+  const int c = 2 * lane;
+  for (int i = 0; i < rows; ++i) {
+    const uint32_t v = *pair_of(stage, i, lane);
+    uint16_t* q = reinterpret_cast<uint16_t*>(p + i * ld + c);
+    if (c + 1 < cols && (reinterpret_cast<uintptr_t>(q) & 3u) == 0) {
+      *reinterpret_cast<uint32_t*>(q) = v;
+    } else {
+      if (c < cols) q[0] = (uint16_t)v;
+      if (c + 1 < cols) q[1] = (uint16_t)(v >> 16);
+    }
   }
+}
+template <typename T>
+__device__ __forceinline__ void rows_in(const T* p, int64_t ld, uint8_t* stage, int lane, int rows, int cols) {
+  const int c = 2 * lane;
+#pragma unroll 8
+  for (int i = 0; i < rows; ++i) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(p + i * ld + c);
+    uint32_t v = 0;
+    if (c + 1 < cols && (reinterpret_cast<uintptr_t>(q) & 3u) == 0) {
+      v = *reinterpret_cast<const uint32_t*>(q);
+    } else {
+      if (c < cols) v = q[0];
+      if (c + 1 < cols) v |= (uint32_t)q[1] << 16;
+    }
+    *pair_of(stage, i, lane) = v;
+  }
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(smem_u32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_read() {  // the stages of this thread's stores are free
+  asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
 }
 
 // Tiles in groups of up to kGroupM rows of tiles, each group column by column:
@@ -111,6 +162,7 @@ __device__ __forceinline__ void tile_at(int t, int tm, int tn, int& m, int& n) {
 template <typename T, int BN, bool AT, bool BT, int ACT>
 __global__ void __launch_bounds__(kThreads, 1)
 k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+       const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_z,
        const Epilogue<T> ep, int slices, int tm, int tn) {
   using L = Ring<BN>;
   constexpr int S = L::kStages;
@@ -215,7 +267,10 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
     }
   } else {
     // ----------------------------------------------------------- epilogue --
-    const int sp = warp & 3, half = (warp - 2) >> 2;  // TMEM lanes 32 sp .., columns half BN / 2 ..
+    // TMEM lanes 32 sp ..; half of the columns (of 64 in all: the first half all)
+    const int sp = warp & 3, half = (warp - 2) >> 2;
+    const int c0 = BN == 64 ? (half ? 64 : 0) : half * (BN / 2), c1 = BN == 64 ? 64 : c0 + BN / 2;
+    uint8_t* stage = smem + S * L::kStage + (warp - 2) * 4096;
     int i = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++i) {
@@ -224,43 +279,69 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       tile_at(t, tm, tn, m, n);
       if (ok) ok = __all_sync(0xffffffffu, wait_or_abort(&acc_full[buf], (unsigned)(i >> 1) & 1u, abort_flag) && !*abort_flag);
       tc_fence_after();
-      const int row = m * kBM + sp * 32 + lane;
-      for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-        uint32_t r[32];
-        if (ok) tmem_ld32(tmem + ((uint32_t)(sp * 32) << 16) + (uint32_t)(buf * BN + c), r);
-        const int col = n * BN + c;
-        if (row >= ep.M || col >= ep.N) continue;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int at = col + 8 * q, left = ep.N - at;
-          if (left <= 0) break;
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = ok ? __uint_as_float(r[8 * q + e]) : CUDART_NAN_F;
-          if (ep.bias) {
-            float b[8];
-            read8(ep.bias + at, ep.wide_bias, left, b);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += b[e];
+      const int row0 = m * kBM + sp * 32, rows = min(32, ep.M - row0);
+#pragma unroll 1
+      for (int c = c0; c < c1; c += 64) {
+        const int col = n * BN + c, cols = min(64, ep.N - col);
+        if (rows <= 0 || cols <= 0) break;
+        // two passes where z is wanted: the accumulator is read for each
+#pragma unroll 1
+        for (int pass = ep.z ? 0 : 1; pass < 2; ++pass) {
+          if (lane == 0) tma_store_read();
+          __syncwarp();
+          const bool res = pass == 1 && ep.residual != nullptr;
+          if (res && !ep.wide_res) {
+            rows_in(ep.residual + (int64_t)row0 * ep.ldr + col, ep.ldr, stage, lane, rows, cols);
+            __syncwarp();
           }
-          if (ep.z) write8(ep.z + (int64_t)row * ep.ldz + at, ep.wide_z, left, v);
-          if constexpr (ACT != kNone) {
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            if (ok) tmem_ld32(tmem + ((uint32_t)(sp * 32) << 16) + (uint32_t)(buf * BN + c + 32 * h), r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = act_of<ACT>(v[e]);
-          }
-          if (ep.residual) {
-            float b[8];
-            read8(ep.residual + (int64_t)row * ep.ldr + at, ep.wide_res, left, b);
+            for (int q = 0; q < 4; ++q) {
+              const int e0 = 32 * h + 8 * q, left = cols - e0;
+              float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += b[e];
+              for (int e = 0; e < 8; ++e) v[e] = ok ? __uint_as_float(r[8 * q + e]) : CUDART_NAN_F;
+              if (ep.bias) {
+                float b[8];
+                read8(ep.bias + col + e0, ep.wide_bias, left, b);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += b[e];
+              }
+              uint4* at = chunk_of(stage, lane, 4 * h + q);
+              if (pass == 1) {
+                if constexpr (ACT != kNone) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) v[e] = act_of<ACT>(v[e]);
+                }
+                if (res) {
+                  float b[8];
+                  if (!ep.wide_res) unpack16<T, 8>(*at, b);
+                  else read8(ep.residual + (int64_t)(row0 + lane) * ep.ldr + col + e0, 1, lane < rows ? left : 0, b);
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) v[e] += b[e];
+                }
+              }
+              *at = pack8<T>(v);
+            }
           }
-          write8(ep.d + (int64_t)row * ep.ldd + at, ep.wide_d, left, v);
+          if (pass == 0 || ep.wide_d) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tma_store_2d(pass == 0 ? &map_z : &map_d, stage, col, row0);
+          } else {
+            __syncwarp();
+            rows_out(ep.d + (int64_t)row0 * ep.ldd + col, ep.ldd, stage, lane, rows, cols);
+          }
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(&acc_empty[buf])) : "memory");
     }
+    if (lane == 0) tma_store_read();
   }
   __syncthreads();
   if (warp == 1) {
@@ -370,17 +451,16 @@ k_few_rows(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_
 }
 
 // ------------------------------------------------------- dz, db, padded rows --
-// dz = dy act'(z) for a tile of kRowsPer rows x 256 columns (8 a thread), and the
+// dz = dy act'(z) for a tile of `per` rows x 256 columns (8 a thread), and the
 // tile's column sums.  dz may be null (no activation, rows as TMA wants them).
-constexpr int kRowsPer = 128;
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256)
 k_act_grad(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ z, int64_t ldz,
-           T* __restrict__ dz, int64_t lddz, float* __restrict__ part, int64_t M, int N, int wide_dy) {
+           T* __restrict__ dz, int64_t lddz, float* __restrict__ part, int64_t M, int N, int per, int wide_dy) {
   __shared__ float red[8][256];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int col = blockIdx.x * 256 + tx * 8, left = N - col;
-  const int64_t m0 = (int64_t)blockIdx.y * kRowsPer, m1 = m0 + kRowsPer < M ? m0 + kRowsPer : M;
+  const int64_t m0 = (int64_t)blockIdx.y * per, m1 = m0 + per < M ? m0 + per : M;
   float sum[8] = {};
   if (left > 0) {
     for (int64_t m = m0 + ty; m < m1; m += 8) {
@@ -487,6 +567,18 @@ int run_gemm(const char* fn, const Matrix& a, const Matrix& b, const Epilogue<T>
   r = make_tensor_map(fn, &mb, dt, b.p, (uint64_t)b.cols, (uint64_t)b.rows, (uint64_t)b.ld * 2, 64,
                       BT ? 64 : BN, CU_TENSOR_MAP_SWIZZLE_128B);
   if (r != MHC_OK) return r;
+  // outputs: 64 columns x 32 rows a store; a map that is not used is the operand's
+  CUtensorMap md = ma, mz = ma;
+  if (ep.wide_d) {
+    r = make_tensor_map(fn, &md, dt, ep.d, (uint64_t)ep.N, (uint64_t)ep.M, (uint64_t)ep.ldd * 2, 64, 32,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r != MHC_OK) return r;
+  }
+  if (ep.z) {
+    r = make_tensor_map(fn, &mz, dt, ep.z, (uint64_t)ep.N, (uint64_t)ep.M, (uint64_t)ep.ldz * 2, 64, 32,
+                        CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r != MHC_OK) return r;
+  }
   const auto kern = k_gemm<T, BN, AT, BT, ACT>;
   const cudaError_t e = allow_dyn_smem(kern, Ring<BN>::kBytes);
   if (e != cudaSuccess) return set_error(MHC_ERR_CUDA, "%s: %s", fn, cudaGetErrorString(e));
@@ -494,7 +586,7 @@ int run_gemm(const char* fn, const Matrix& a, const Matrix& b, const Epilogue<T>
   if ((int64_t)tm * tn > 0x7fffffff - 65536)
     return set_error(MHC_ERR_UNSUPPORTED, "%s: %d x %d outputs are too many", fn, ep.M, ep.N);
   const int grid = tm * tn < sm_count() ? tm * tn : sm_count();
-  kern<<<grid, kThreads, Ring<BN>::kBytes, st>>>(ma, mb, ep, (int)((red + kBK - 1) / kBK), tm, tn);
+  kern<<<grid, kThreads, Ring<BN>::kBytes, st>>>(ma, mb, md, mz, ep, (int)((red + kBK - 1) / kBK), tm, tn);
   return check_launch(fn);
 }
 // The tile width with the least time by waves of tiles: a 128 x 256 tile takes
@@ -526,6 +618,13 @@ int gemm(const char* fn, const Matrix& a, const Matrix& b, const Epilogue<T>& ep
 }
 
 constexpr int kFewRows = 16;
+// Rows to a block of k_act_grad: 128, fewer (down to 16) while there are not two
+// blocks an SM.
+int rows_per(int64_t M, int64_t N) {
+  int per = 128;
+  while (per > 16 && (M + per - 1) / per * ((N + 255) / 256) < 2 * (int64_t)sm_count()) per /= 2;
+  return per;
+}
 
 template <typename T>
 Epilogue<T> epilogue(void* d, int64_t ldd, int64_t M, int64_t N) {
@@ -549,7 +648,6 @@ int forward(const LinearArg& l, cudaStream_t st) {
   ep.ldz = l.ldz;
   ep.wide_bias = aligned16(l.bias);
   ep.wide_res = tma_rows(l.residual, l.ldr);
-  ep.wide_z = tma_rows(l.z, l.ldz);
   if (l.M <= kFewRows) {
     const bool aligned = tma_rows(l.x, l.ldx) && tma_rows(l.w, l.ldw) && l.K % 8 == 0;
     const unsigned grid = (unsigned)((l.N + 15) / 16);
@@ -584,7 +682,8 @@ int backward(const LinearGradArg& l, cudaStream_t st) {
       q = ws.take(padded_bytes(l.M, l.N));
       if (!q) return no_space(fn);
     }
-    const int64_t parts = (l.M + kRowsPer - 1) / kRowsPer;
+    const int per = rows_per(l.M, l.N);
+    const int64_t parts = (l.M + per - 1) / per;
     float* part = nullptr;
     if (l.dbias) {
       part = static_cast<float*>(ws.take((size_t)parts * (size_t)l.N * sizeof(float)));
@@ -593,7 +692,7 @@ int backward(const LinearGradArg& l, cudaStream_t st) {
     if (parts > 65535) return set_error(MHC_ERR_UNSUPPORTED, "%s: M=%lld is too large", fn, (long long)l.M);
     const dim3 grid((unsigned)((l.N + 255) / 256), (unsigned)parts);
     k_act_grad<T, ACT><<<grid, 256, 0, st>>>(static_cast<const T*>(l.dy), l.ldy, static_cast<const T*>(l.z),
-                                             l.ldz, static_cast<T*>(q), up8(l.N), part, l.M, (int)l.N,
+                                             l.ldz, static_cast<T*>(q), up8(l.N), part, l.M, (int)l.N, per,
                                              tma_rows(l.dy, l.ldy));
     int r = check_launch(fn);
     if (r != MHC_OK) return r;
@@ -638,7 +737,10 @@ size_t linear_fwd_ws_bytes(const void* x, int64_t ldx, const void* w, int64_t ld
 size_t linear_bwd_ws_bytes(const LinearGradArg& l) {
   size_t n = 0;
   if ((l.dx || l.dw) && (l.act != kNone || !tma_rows(l.dy, l.ldy))) n += padded_bytes(l.M, l.N);
-  if (l.dbias) n += up256((size_t)((l.M + kRowsPer - 1) / kRowsPer) * (size_t)l.N * sizeof(float));
+  if (l.dbias) {
+    const int per = rows_per(l.M, l.N);
+    n += up256((size_t)((l.M + per - 1) / per) * (size_t)l.N * sizeof(float));
+  }
   if (l.dx && !tma_rows(l.w, l.ldw)) n += padded_bytes(l.N, l.K);
   if (l.dw && !tma_rows(l.x, l.ldx)) n += padded_bytes(l.M, l.K);
   return n;

@@ -170,7 +170,7 @@ def exported_symbols() -> list[str]:
 def call(name: str, *args) -> None:
     """Call a status-returning entry point; raise on a nonzero status."""
     global CALLS
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     CALLS += 1
     if rc != MHC_OK:

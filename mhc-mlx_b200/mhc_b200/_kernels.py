@@ -38,6 +38,9 @@ def _timed(name: str, ref: torch.Tensor):
 
 def _call(name: str, ref: torch.Tensor, *args) -> None:
     """C.call with optional per-launch event timing (see TIMING)."""
+    if TIMING is None:
+        C.call(name, *args)
+        return
     with _timed(name, ref):
         C.call(name, *args)
 
@@ -487,20 +490,21 @@ class LogitRows:
 
     def __init__(self, logits: torch.Tensor, targets: torch.Tensor, ignore_index: int):
         self.dev = C.require_cuda(logits, targets)
-        V = logits.shape[-1]
-        if logits.stride(-1) != 1 and V > 1:
+        strides, V = logits.stride(), logits.shape[-1]
+        if strides[-1] != 1 and V > 1:
             logits = logits.contiguous()
+            strides = logits.stride()
         self.logits, self.targets = logits, _c(targets)
         self.shape, self.rows = targets.shape, targets.numel()
-        if logits.ndim == 3:
-            per, sb, sr = logits.shape[1], logits.stride(0), logits.stride(1)
+        if len(strides) == 3:
+            per, sb, sr = logits.shape[1], strides[0], strides[1]
         else:
-            per, sb, sr = self.rows, 0, logits.stride(0)
-        self.args = (C.ptr(logits), C.dtype_code(logits.dtype), self.rows, max(per, 1), sb, sr, V,
-                     C.ptr(self.targets), ignore_index)
+            per, sb, sr = self.rows, 0, strides[0]
+        self.args = (logits.data_ptr(), C.dtype_code(logits.dtype), self.rows, max(per, 1), sb, sr,
+                     V, self.targets.data_ptr(), ignore_index)
 
     def grad_like(self) -> torch.Tensor:
-        return torch.empty(self.logits.shape, dtype=self.logits.dtype, device=self.dev)
+        return self.logits.new_empty(self.logits.shape)
 
     def floats(self, *shape) -> torch.Tensor:
         return torch.empty(*shape, dtype=F32, device=self.dev)
@@ -529,40 +533,54 @@ def logits_grad(r: LogitRows, stats, coef, scale=None, ready=None):
     return out
 
 
+def _row_records(r: LogitRows, like: torch.Tensor):
+    """(stats, coef) of a loss: five floats a row in one buffer."""
+    rows = r.rows
+    both = like.new_empty(5 * rows)
+    return both, both.data_ptr(), both.data_ptr() + 16 * rows
+
+
+def split_records(both: torch.Tensor):
+    """(stats [rows, 4], coef [rows]) of a loss's records."""
+    rows = both.numel() // 5
+    return both[:4 * rows].view(rows, 4), both[4 * rows:]
+
+
 def preference_loss(r: LogitRows, ref, cu, pairs: int, beta: float, smoothing: float,
                     inv_d: float, grad_scale: float, want_grad: bool):
-    """(loss, logp, margins, dlogits or None, stats, coef)"""
+    """(loss, logp, margins, dlogits or None, records)"""
     C.require_cuda(r.logits, ref, cu)
     with _on(r.dev):
         ref = _f32(ref)
         cu = None if cu is None else _c(cu)
         uniform = r.logits.shape[1] if cu is None else 0
-        loss, margins, logp = r.floats(()), r.floats(pairs), r.floats(r.shape)
-        stats, coef = r.floats(r.rows, 4), r.floats(r.rows)
+        loss, margins, logp = ref.new_empty(()), ref.new_empty(pairs), ref.new_empty(r.shape)
+        both, stats, coef = _row_records(r, ref)
         dlogits = r.grad_like() if want_grad else None
         _call("mhc_preference_loss", r.logits, *r.args, C.ptr(cu),
-              int(cu is not None and cu.dtype == torch.int64), uniform, pairs, C.ptr(ref), beta,
-              smoothing, inv_d, grad_scale, C.ptr(logp), C.ptr(stats), C.ptr(coef),
-              C.ptr(margins), C.ptr(loss), C.ptr(dlogits), C.stream_of(r.logits))
-    return loss, logp, margins, dlogits, stats, coef
+              int(cu is not None and cu.dtype == torch.int64), uniform, pairs, ref.data_ptr(), beta,
+              smoothing, inv_d, grad_scale, logp.data_ptr(), stats, coef, margins.data_ptr(),
+              loss.data_ptr(), C.ptr(dlogits), C.stream_of(r.logits))
+    return loss, logp, margins, dlogits, both
 
 
 def policy_loss(r: LogitRows, old, adv, ref, clip_low: float, clip_high: float, kl_coef: float,
                 inv_d: float, grad_scale: float, want_grad: bool):
-    """(loss, logp, kl, dlogits or None, stats, coef)"""
+    """(loss, logp, kl, dlogits or None, records)"""
     C.require_cuda(r.logits, old, adv, ref)
     with _on(r.dev):
         old, adv = _f32(old), _f32(adv)
         ref = None if ref is None else _f32(ref)
-        loss, kl, logp = r.floats(()), r.floats(()), r.floats(r.shape)
-        stats, coef = r.floats(r.rows, 4), r.floats(r.rows)
+        loss, kl, logp = old.new_empty(()), old.new_empty(()), old.new_empty(r.shape)
+        both, stats, coef = _row_records(r, old)
         dlogits = r.grad_like() if want_grad else None
         nb = _ws_bytes("mhc_policy_workspace_bytes", r.dev)
         ws = _ws(nb, r.dev)
-        _call("mhc_policy_loss", r.logits, *r.args, C.ptr(old), C.ptr(adv), C.ptr(ref), clip_low,
-              clip_high, kl_coef, inv_d, grad_scale, C.ptr(logp), C.ptr(stats), C.ptr(coef),
-              C.ptr(loss), C.ptr(kl), C.ptr(dlogits), C.ptr(ws), nb, C.stream_of(r.logits))
-    return loss, logp, kl, dlogits, stats, coef
+        _call("mhc_policy_loss", r.logits, *r.args, old.data_ptr(), adv.data_ptr(), C.ptr(ref),
+              clip_low, clip_high, kl_coef, inv_d, grad_scale, logp.data_ptr(), stats, coef,
+              loss.data_ptr(), kl.data_ptr(), C.ptr(dlogits), ws.data_ptr(), nb,
+              C.stream_of(r.logits))
+    return loss, logp, kl, dlogits, both
 
 
 # ------------------------------------------------------------------ AdamW --

@@ -71,8 +71,12 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     fp32, rounded once to y.  The gradients are rounded once to their tensors'
     type; with an activation the pre-activation (kept for the backward) and its
     gradient (an operand of the products) are rounded to the type too."""
-    return _LinearFn.apply(x, weight, bias, residual,
-                           _check(x, weight, bias, residual, activation))
+    act = _check(x, weight, bias, residual, activation)
+    if not torch.is_grad_enabled() or not any(
+            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        # a decoding step: nothing to record
+        return K.linear_fwd(x, weight, bias, residual, act, keep_z=False)[0]
+    return _LinearFn.apply(x, weight, bias, residual, act)
 
 
 class FusedLinear(nn.Linear):

@@ -146,9 +146,9 @@ class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ref, cu, pairs, beta, smoothing, inv_d, ignore_index):
         rows = K.LogitRows(logits, targets, ignore_index)
-        loss, logp, margins, _, stats, coef = K.preference_loss(
+        loss, logp, margins, _, records = K.preference_loss(
             rows, ref, cu, pairs, beta, smoothing, inv_d, 1.0, want_grad=False)
-        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.save_for_backward(logits, targets, records)
         ctx.ignore_index = ignore_index
         ctx.mark_non_differentiable(logp, margins)
         return loss, logp, margins
@@ -156,8 +156,9 @@ class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d, _logp, _margins):
-        logits, targets, stats, coef = ctx.saved_tensors
+        logits, targets, records = ctx.saved_tensors
         rows = K.LogitRows(logits, targets, ctx.ignore_index)
+        stats, coef = K.split_records(records)
         return (K.logits_grad(rows, stats, coef, scale=d),) + (None,) * 8
 
 
@@ -191,8 +192,8 @@ def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor, ref_logpro
     """``preference_loss`` and, in ``dlogits``, grad_scale times its gradient."""
     pairs, inv_d = _check_preference(logits, targets, ref_logprobs, cu_seqlens, label_smoothing,
                                      denominator)
-    rows = K.LogitRows(logits.detach(), targets, int(ignore_index))
-    loss, logp, margins, dlogits, _, _ = K.preference_loss(
+    rows = K.LogitRows(logits, targets, int(ignore_index))
+    loss, logp, margins, dlogits, _ = K.preference_loss(
         rows, ref_logprobs, cu_seqlens, pairs, float(beta), float(label_smoothing), inv_d,
         float(grad_scale), want_grad=True)
     return PreferenceResult(loss, logp, margins, dlogits)
@@ -207,9 +208,9 @@ class _PolicyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, old, adv, ref, lo, hi, kl_coef, inv_d, ignore_index):
         rows = K.LogitRows(logits, targets, ignore_index)
-        loss, logp, kl, dlogits, stats, coef = K.policy_loss(
+        loss, logp, kl, dlogits, records = K.policy_loss(
             rows, old, adv, ref, lo, hi, kl_coef, inv_d, 1.0, want_grad=ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.save_for_backward(logits, targets, records)
         ctx.ignore_index, ctx.dlogits = ignore_index, dlogits
         ctx.mark_non_differentiable(logp, kl)
         return loss, logp, kl
@@ -217,8 +218,9 @@ class _PolicyFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d, _logp, _kl):
-        logits, targets, stats, coef = ctx.saved_tensors
+        logits, targets, records = ctx.saved_tensors
         rows = K.LogitRows(logits, targets, ctx.ignore_index)
+        stats, coef = K.split_records(records)
         # handed over once: a second backward over a kept graph computes its own
         ready, ctx.dlogits = ctx.dlogits, None
         return (K.logits_grad(rows, stats, coef, scale=d, ready=ready),) + (None,) * 9
@@ -252,8 +254,8 @@ def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: 
     """``policy_loss`` and, in ``dlogits``, grad_scale times its gradient."""
     inv_d = _check_policy(logits, targets, old_logprobs, advantages, ref_logprobs, clip_low,
                           clip_high, kl_coef, denominator)
-    rows = K.LogitRows(logits.detach(), targets, int(ignore_index))
-    loss, logp, kl, dlogits, _, _ = K.policy_loss(
+    rows = K.LogitRows(logits, targets, int(ignore_index))
+    loss, logp, kl, dlogits, _ = K.policy_loss(
         rows, old_logprobs, advantages, ref_logprobs, float(clip_low), float(clip_high),
         float(kl_coef), inv_d, float(grad_scale), want_grad=True)
     return PolicyResult(loss, logp, kl, dlogits)

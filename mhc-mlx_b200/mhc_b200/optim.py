@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from operator import attrgetter
 
 import torch
@@ -58,7 +59,6 @@ class _Pack:
         self.offsets, self.total = offsets, total
         self.numel = (ctypes.c_int64 * n)(*sizes)
         self.off = (ctypes.c_int64 * n)(*offsets)
-        self.p_ptr, self.g_ptr = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)()
         # every gradient must lie in memory as its parameter does
         self.plain = all(p.is_contiguous() for p in params)
         zeros = lambda k, dt: torch.zeros(max(k, 1), dtype=dt, device=self.device)[:k]  # noqa: E731
@@ -119,10 +119,9 @@ class _Pack:
         self.steps = [t] * len(grads)
         if self.total == 0:
             return
-        self.p_ptr[:] = list(map(_data_ptr, self.params))
-        self.g_ptr[:] = list(map(_data_ptr, grads))
-        self._call(group, t, seed, grad_scale, len(grads), self.p_ptr, self.g_ptr, self.numel,
-                   self.off)
+        p_ptr, g_ptr = array("Q", map(_data_ptr, self.params)), array("Q", map(_data_ptr, grads))
+        self._call(group, t, seed, grad_scale, len(grads), p_ptr.buffer_info()[0],
+                   g_ptr.buffer_info()[0], self.numel, self.off)
 
     @staticmethod
     def _as_param(p, g):
