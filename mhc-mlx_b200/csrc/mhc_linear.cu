@@ -80,7 +80,7 @@ struct Epilogue {
   T* d;               // [M][ldd]
   int64_t ldr, ldz, ldd;
   int M, N;
-  int wide_bias, wide_res, wide_d;  // 16-byte accesses are possible
+  int wide_res, wide_d;  // 16-byte accesses are possible
 };
 
 // Up to 8 consecutive values from p as fp32, 0 past n.
@@ -277,20 +277,43 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       const int buf = i & 1;
       int m, n;
       tile_at(t, tm, tn, m, n);
+      const int row0 = m * kBM + sp * 32, rows = min(32, ep.M - row0);
+      // what does not hang on the products comes while they run: the bias, and the
+      // residual (its first 64 columns into the stage, or all of it into L2)
+      float bias[4] = {};  // of columns c0 + lane, + 32, + 64, + 96
+      if (ep.bias) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int c = c0 + 32 * k + lane;
+          if (c < c1 && n * BN + c < ep.N) bias[k] = to_f(ep.bias[n * BN + c]);
+        }
+      }
+      if (ep.residual && rows > 0) {
+        if (!ep.wide_res) {
+          if (lane == 0) tma_store_read();
+          __syncwarp();
+          if (c0 < c1) rows_in(ep.residual + (int64_t)row0 * ep.ldr + n * BN + c0, ep.ldr, stage, lane, rows, ep.N - n * BN - c0);
+        } else if (lane < rows) {
+          for (int c = n * BN + c0; c < n * BN + c1 && c < ep.N; c += 64)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(ep.residual + (int64_t)(row0 + lane) * ep.ldr + c));
+        }
+      }
+      __syncwarp();
       if (ok) ok = __all_sync(0xffffffffu, wait_or_abort(&acc_full[buf], (unsigned)(i >> 1) & 1u, abort_flag) && !*abort_flag);
       tc_fence_after();
-      const int row0 = m * kBM + sp * 32, rows = min(32, ep.M - row0);
 #pragma unroll 1
       for (int c = c0; c < c1; c += 64) {
         const int col = n * BN + c, cols = min(64, ep.N - col);
         if (rows <= 0 || cols <= 0) break;
-        // two passes where z is wanted: the accumulator is read for each
+        // y, then z where it is wanted: the accumulator is read for each
 #pragma unroll 1
-        for (int pass = ep.z ? 0 : 1; pass < 2; ++pass) {
-          if (lane == 0) tma_store_read();
-          __syncwarp();
-          const bool res = pass == 1 && ep.residual != nullptr;
-          if (res && !ep.wide_res) {
+        for (int pass = 0; pass < (ep.z ? 2 : 1); ++pass) {
+          const bool res = pass == 0 && ep.residual != nullptr, staged = res && !ep.wide_res;
+          if (!staged || c != c0) {
+            if (lane == 0) tma_store_read();
+            __syncwarp();
+          }
+          if (staged && c != c0) {
             rows_in(ep.residual + (int64_t)row0 * ep.ldr + col, ep.ldr, stage, lane, rows, cols);
             __syncwarp();
           }
@@ -298,28 +321,27 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
           for (int h = 0; h < 2; ++h) {
             uint32_t r[32];
             if (ok) tmem_ld32(tmem + ((uint32_t)(sp * 32) << 16) + (uint32_t)(buf * BN + c + 32 * h), r);
+            const float bl = c == c0 ? (h ? bias[1] : bias[0]) : (h ? bias[3] : bias[2]);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              const int e0 = 32 * h + 8 * q, left = cols - e0;
+              const int e0 = 32 * h + 8 * q;
               float v[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) v[e] = ok ? __uint_as_float(r[8 * q + e]) : CUDART_NAN_F;
               if (ep.bias) {
-                float b[8];
-                read8(ep.bias + col + e0, ep.wide_bias, left, b);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += b[e];
+                for (int e = 0; e < 8; ++e) v[e] += __shfl_sync(0xffffffffu, bl, 8 * q + e);
               }
               uint4* at = chunk_of(stage, lane, 4 * h + q);
-              if (pass == 1) {
+              if (pass == 0) {
                 if constexpr (ACT != kNone) {
 #pragma unroll
                   for (int e = 0; e < 8; ++e) v[e] = act_of<ACT>(v[e]);
                 }
                 if (res) {
                   float b[8];
-                  if (!ep.wide_res) unpack16<T, 8>(*at, b);
-                  else read8(ep.residual + (int64_t)(row0 + lane) * ep.ldr + col + e0, 1, lane < rows ? left : 0, b);
+                  if (staged) unpack16<T, 8>(*at, b);
+                  else read8(ep.residual + (int64_t)(row0 + lane) * ep.ldr + col + e0, 1, lane < rows ? cols - e0 : 0, b);
 #pragma unroll
                   for (int e = 0; e < 8; ++e) v[e] += b[e];
                 }
@@ -327,13 +349,14 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
               *at = pack8<T>(v);
             }
           }
-          if (pass == 0 || ep.wide_d) {
+          if (pass == 1 || ep.wide_d) {
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) tma_store_2d(pass == 0 ? &map_z : &map_d, stage, col, row0);
+            if (lane == 0) tma_store_2d(pass == 1 ? &map_z : &map_d, stage, col, row0);
           } else {
             __syncwarp();
             rows_out(ep.d + (int64_t)row0 * ep.ldd + col, ep.ldd, stage, lane, rows, cols);
+            __syncwarp();
           }
         }
       }
@@ -391,7 +414,7 @@ template <typename T, int MT, int ACT, bool ALIGNED>
 __global__ void __launch_bounds__(256)
 k_few_rows(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
            const Epilogue<T> ep, int K) {
-  constexpr int kU = MT == 1 ? 4 : 2;  // slices in flight
+  constexpr int kU = MT == 1 ? 6 : 3;  // slices in flight
   __shared__ float part[8][16][8 * MT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, q = lane & 3;
@@ -502,17 +525,26 @@ k_bias_sum(const float* __restrict__ part, int rows, int N, T* __restrict__ db) 
   for (int r = 0; r < rows; ++r) s += part[(int64_t)r * N + c];
   db[c] = from_f<T>(s);
 }
-// Rows of `cols` values at stride ld -> rows padded with zeros to ldp.
+// Rows of `cols` values at stride ld -> rows padded with zeros to ldp: one or two
+// matrices in a launch.
+template <typename T>
+struct Pad {
+  const T* src;
+  T* dst;
+  int64_t ld, ldp, rows;
+  int cols;
+};
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_pad(const T* __restrict__ src, int64_t ld, int64_t rows, int cols, T* __restrict__ dst, int64_t ldp) {
-  const int64_t per = ldp / 8, total = rows * per;
+k_pad(const Pad<T> a, const Pad<T> b) {
+  const int64_t na = a.rows * (a.ldp / 8), total = na + b.rows * (b.ldp / 8);
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = i / per;
-    const int c = (int)(i - m * per) * 8;
+    const Pad<T>& p = i < na ? a : b;
+    const int64_t j = i < na ? i : i - na, per = p.ldp / 8, m = j / per;
+    const int c = (int)(j - m * per) * 8;
     float v[8];
-    read8(src + m * ld + c, false, cols - c, v);
-    store_vec<T, 8, false>(dst + m * ldp + c, v);
+    read8(p.src + m * p.ld + c, false, p.cols - c, v);
+    store_vec<T, 8, false>(p.dst + m * p.ldp + c, v);
   }
 }
 
@@ -540,18 +572,27 @@ struct Matrix {  // rows x cols values, rows ld apart
   const void* p;
   int64_t rows, cols, ld;
 };
+// The matrices (either may be null) with rows that TMA can read: padded copies
+// where they are not.
 template <typename T>
-int for_tma(const char* fn, Matrix& a, Space& ws, cudaStream_t st) {
-  if (tma_rows(a.p, a.ld)) return MHC_OK;
-  const int64_t ldp = up8(a.cols);
-  void* q = ws.take(padded_bytes(a.rows, a.cols));
-  if (!q) return no_space(fn);
-  int64_t blocks = (a.rows * (ldp / 8) + 255) / 256;
+int for_tma(const char* fn, Matrix* a, Matrix* b, Space& ws, cudaStream_t st) {
+  Pad<T> p[2] = {};
+  int64_t work = 0;
+  int n = 0;
+  for (Matrix* m : {a, b}) {
+    if (!m || tma_rows(m->p, m->ld)) continue;
+    void* q = ws.take(padded_bytes(m->rows, m->cols));
+    if (!q) return no_space(fn);
+    const int64_t ldp = up8(m->cols);
+    p[n++] = {static_cast<const T*>(m->p), static_cast<T*>(q), m->ld, ldp, m->rows, (int)m->cols};
+    work += m->rows * (ldp / 8);
+    m->p = q;
+    m->ld = ldp;
+  }
+  if (n == 0) return MHC_OK;
+  int64_t blocks = (work + 255) / 256;
   if (blocks > (int64_t)sm_count() * 16) blocks = (int64_t)sm_count() * 16;
-  k_pad<T><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const T*>(a.p), a.ld, a.rows, (int)a.cols,
-                                             static_cast<T*>(q), ldp);
-  a.p = q;
-  a.ld = ldp;
+  k_pad<T><<<(unsigned)blocks, 256, 0, st>>>(p[0], p[1]);
   return check_launch(fn);
 }
 
@@ -646,7 +687,6 @@ int forward(const LinearArg& l, cudaStream_t st) {
   ep.ldr = l.ldr;
   ep.z = static_cast<T*>(l.z);
   ep.ldz = l.ldz;
-  ep.wide_bias = aligned16(l.bias);
   ep.wide_res = tma_rows(l.residual, l.ldr);
   if (l.M <= kFewRows) {
     const bool aligned = tma_rows(l.x, l.ldx) && tma_rows(l.w, l.ldw) && l.K % 8 == 0;
@@ -664,8 +704,7 @@ int forward(const LinearArg& l, cudaStream_t st) {
   }
   Space ws = {static_cast<char*>(l.workspace), static_cast<char*>(l.workspace) + l.workspace_bytes};
   Matrix a = {l.x, l.M, l.K, l.ldx}, b = {l.w, l.N, l.K, l.ldw};
-  int r = for_tma<T>(fn, a, ws, st);
-  if (r == MHC_OK) r = for_tma<T>(fn, b, ws, st);
+  const int r = for_tma<T>(fn, &a, &b, ws, st);
   return r != MHC_OK ? r : gemm<T, false, false, ACT>(fn, a, b, ep, l.K, st);
 }
 
@@ -704,19 +743,13 @@ int backward(const LinearGradArg& l, cudaStream_t st) {
     }
     if (own) dz = {q, l.M, l.N, up8(l.N)};
   }
-  if (l.dx) {  // dx[m, k] = sum_n dz[m, n] W[n, k]
-    Matrix w = {l.w, l.N, l.K, l.ldw};
-    int r = for_tma<T>(fn, w, ws, st);
-    if (r == MHC_OK) r = gemm<T, false, true, kNone>(fn, dz, w, epilogue<T>(l.dx, l.lddx, l.M, l.K), l.N, st);
-    if (r != MHC_OK) return r;
-  }
-  if (l.dw) {  // dW[n, k] = sum_m dz[m, n] x[m, k]
-    Matrix x = {l.x, l.M, l.K, l.ldx};
-    int r = for_tma<T>(fn, x, ws, st);
-    if (r == MHC_OK) r = gemm<T, true, true, kNone>(fn, dz, x, epilogue<T>(l.dw, l.lddw, l.N, l.K), l.M, st);
-    if (r != MHC_OK) return r;
-  }
-  return MHC_OK;
+  Matrix w = {l.w, l.N, l.K, l.ldw}, x = {l.x, l.M, l.K, l.ldx};
+  int r = for_tma<T>(fn, l.dx ? &w : nullptr, l.dw ? &x : nullptr, ws, st);
+  if (r == MHC_OK && l.dx)  // dx[m, k] = sum_n dz[m, n] W[n, k]
+    r = gemm<T, false, true, kNone>(fn, dz, w, epilogue<T>(l.dx, l.lddx, l.M, l.K), l.N, st);
+  if (r == MHC_OK && l.dw)  // dW[n, k] = sum_m dz[m, n] x[m, k]
+    r = gemm<T, true, true, kNone>(fn, dz, x, epilogue<T>(l.dw, l.lddw, l.N, l.K), l.M, st);
+  return r;
 }
 
 #define MHC_BY_ACT(F, T, l, st)                 \

@@ -598,21 +598,19 @@ def adamw_step(dev: torch.device, count: int, params, grads, numel, offsets, dty
 
 
 # ----------------------------------------------------------------- linear --
-def _rows2d(t: torch.Tensor) -> torch.Tensor:
-    """[..., C] as [rows, C] with contiguous rows, in place where its strides allow."""
+def _rows(t: torch.Tensor):
+    """(t, distance between its rows) of [..., C] taken as [rows, C]: in place where
+    its strides allow, else a copy."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         t = t.contiguous()
-    return t.reshape(-1, t.shape[-1])
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Distance between the rows of a 2-D tensor (of one row: its length)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _spread(t: torch.Tensor) -> torch.Tensor:
-    """Rows that overlap (an expanded tensor) cannot be walked: copied."""
-    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
+    t = t.reshape(-1, t.shape[-1])
+    if t.shape[0] <= 1:
+        return t, t.shape[1]
+    if t.stride(0) < t.shape[1]:  # rows that overlap (an expanded tensor)
+        t = t.contiguous()
+    return t, t.stride(0)
 
 
 def linear_fwd(x, weight, bias, residual, act: int, keep_z: bool):
@@ -620,18 +618,20 @@ def linear_fwd(x, weight, bias, residual, act: int, keep_z: bool):
     dev = C.require_cuda(x, weight, bias, residual)
     N, Kc = weight.shape
     with _on(dev):
-        x2, w2 = _spread(_rows2d(x)), _spread(_rows2d(weight))
-        M = x2.shape[0]
-        r2 = None if residual is None else _spread(_rows2d(residual))
+        M = x.numel() // Kc
+        (x2, ldx), (w2, ldw) = _rows(x), _rows(weight)
+        r2, ldr = (None, 0) if residual is None else _rows(residual)
         b1 = None if bias is None else _c(bias)
-        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=dev)
+        y = x.new_empty(*x.shape[:-1], N)
         ldz = (N + 7) // 8 * 8
-        z = torch.empty(M, ldz, dtype=x.dtype, device=dev) if keep_z else None
-        args = (C.ptr(x2), _ld(x2), C.ptr(w2), _ld(w2))
-        nb = int(C.query("mhc_linear_fwd_workspace_bytes", *args, M, N, Kc))
-        ws = _ws(nb, dev) if nb else None
-        _call("mhc_linear_fwd", x2, *args, C.ptr(b1), C.ptr(r2), 0 if r2 is None else _ld(r2),
-              C.dtype_code(x.dtype), act, C.ptr(z), ldz, C.ptr(y), N, M, N, Kc, C.ptr(ws), nb,
+        z = x.new_empty(M, ldz) if keep_z else None
+        px, pw = x2.data_ptr(), w2.data_ptr()
+        nb, ws = 0, None
+        if (px | pw | 2 * ldx | 2 * ldw) & 15:  # rows that need padded copies
+            nb = int(C.query("mhc_linear_fwd_workspace_bytes", px, ldx, pw, ldw, M, N, Kc))
+            ws = _ws(nb, dev) if nb else None
+        _call("mhc_linear_fwd", x2, px, ldx, pw, ldw, C.ptr(b1), C.ptr(r2), ldr,
+              C.dtype_code(x.dtype), act, C.ptr(z), ldz, y.data_ptr(), N, M, N, Kc, C.ptr(ws), nb,
               C.stream_of(x2))
     return y, z
 
@@ -641,18 +641,16 @@ def linear_bwd(dy, z, x, weight, act: int, want_dx: bool, want_dw: bool, want_db
     dev = C.require_cuda(dy, x, weight)
     N, Kc = weight.shape
     with _on(dev):
-        d2, x2, w2 = _spread(_rows2d(dy)), _spread(_rows2d(x)), _spread(_rows2d(weight))
-        M = x2.shape[0]
-        new = lambda *s: torch.empty(*s, dtype=x.dtype, device=dev)  # noqa: E731
-        dx = new(*x.shape) if want_dx else None
-        dw = new(N, Kc) if want_dw else None
-        db = new(N) if want_db else None
-        args = (C.ptr(d2), _ld(d2))
-        ops = (C.ptr(x2), _ld(x2), C.ptr(w2), _ld(w2))
-        nb = int(C.query("mhc_linear_bwd_workspace_bytes", *args, *ops, act, int(want_dx),
-                         int(want_dw), int(want_db), M, N, Kc))
+        M = x.numel() // Kc
+        (d2, ldd), (x2, ldx), (w2, ldw) = _rows(dy), _rows(x), _rows(weight)
+        dx = x.new_empty(x.shape) if want_dx else None
+        dw = x.new_empty(N, Kc) if want_dw else None
+        db = x.new_empty(N) if want_db else None
+        pd, px, pw = d2.data_ptr(), x2.data_ptr(), w2.data_ptr()
+        nb = int(C.query("mhc_linear_bwd_workspace_bytes", pd, ldd, px, ldx, pw, ldw, act, want_dx,
+                         want_dw, want_db, M, N, Kc))
         ws = _ws(nb, dev) if nb else None
-        _call("mhc_linear_bwd", x2, *args, C.ptr(z), 0 if z is None else z.shape[1], *ops,
-              C.dtype_code(x.dtype), act, C.ptr(dx), Kc, C.ptr(dw), Kc, C.ptr(db), M, N, Kc,
+        _call("mhc_linear_bwd", x2, pd, ldd, C.ptr(z), 0 if z is None else z.shape[1], px, ldx, pw,
+              ldw, C.dtype_code(x.dtype), act, C.ptr(dx), Kc, C.ptr(dw), Kc, C.ptr(db), M, N, Kc,
               C.ptr(ws), nb, C.stream_of(x2))
     return dx, dw, db
