@@ -15,7 +15,8 @@ import sys as _sys
 from mhc_b200 import (AutoPatcher, MHCLayer, MHCRewire, QuantizedLinear, __version__,  # noqa: F401
                       diagnostics, residual_add_agg)
 
-for _name in ("metal", "layer", "patching", "utils", "quantized", "dist"):
+for _name in ("metal", "layer", "patching", "utils", "quantized", "dist", "losses", "optim",
+              "linear"):
     _mod = _importlib.import_module(f"mhc_b200.{_name}")
     _sys.modules[f"{__name__}.{_name}"] = _mod
     globals()[_name] = _mod
