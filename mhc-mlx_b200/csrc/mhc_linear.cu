@@ -411,10 +411,10 @@ __device__ __forceinline__ uint4 eight_at(const uint16_t* row, int k, int K) {
 // warps take every eighth slice of 32 k; their sums meet in shared memory, in
 // order.
 template <typename T, int MT, int ACT, bool ALIGNED>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 k_few_rows(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw,
            const Epilogue<T> ep, int K) {
-  constexpr int kU = MT == 1 ? 6 : 3;  // slices in flight
+  constexpr int kU = MT == 1 ? 8 : 4;  // slices in flight
   __shared__ float part[8][16][8 * MT + 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, q = lane & 3;

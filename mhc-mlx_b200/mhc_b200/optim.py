@@ -43,6 +43,22 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+class _States(dict):
+    """Optimizer.state: a parameter's views of the flat buffers are made when they are
+    first asked for (hundreds of parameters, four buffers each)."""
+
+    def __init__(self, owner):
+        super().__init__()
+        self.owner, self.where = owner, {}
+
+    def __missing__(self, p):
+        if p not in self.where:  # a group has been added
+            self.where = self.owner._where()
+        pack, i = self.where[p]
+        self[p] = pack.state_of(i)
+        return self[p]
+
+
 class _Pack:
     """The parameters of one group that share a type and a device, and their state."""
 
@@ -166,6 +182,7 @@ class AdamW(torch.optim.Optimizer):
         self.seed = int(seed)
         self._packs: list[list[_Pack]] = []
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.state = _States(self)
 
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
@@ -192,8 +209,6 @@ class AdamW(torch.optim.Optimizer):
         for k, ((dtype, _), ps) in enumerate(by.items()):
             pack = _Pack(ps, self.state_bits, self.master_weights and dtype != torch.float32,
                          64 * index + k)
-            for i, p in enumerate(ps):
-                self.state[p] = pack.state_of(i)
             packs.append(pack)
         return packs
 

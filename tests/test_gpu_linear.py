@@ -74,9 +74,10 @@ def _check(x, w, b, res, dy, act, y, grads):
 
 # tokens: each side of the few-rows kernel (8, 16), of a tile (128); widths: one
 # tile column of 64, ragged, odd (padded rows), several waves of the widest tile
+# (in all three products)
 SIZES = [(1, 64, 64), (1, 1500, 1001), (5, 17, 8), (8, 333, 4096), (9, 128, 40), (16, 100, 96),
          (17, 64, 64), (100, 1, 1), (130, 257, 100), (129, 72, 8), (300, 1000, 333), (77, 1500, 1001),
-         (1500, 2600, 700), (2048, 4096, 264)]
+         (1500, 2600, 700), (2048, 4096, 264), (2300, 2040, 2000), (2300, 2042, 1999)]
 
 
 @pytest.mark.parametrize("dtype", list(U))
