@@ -29,6 +29,13 @@
 // a block, its eight warps splitting K, with warp-level MMAs (a tensor-memory
 // tile would be empty but for 1/8 of it).  Operands whose rows do not begin on
 // 16-byte boundaries, which TMA cannot read, are copied to padded rows first.
+//
+// Measured, bf16, 8192 rows, 4096 to 11008, bias and SiLU: y 537 us,
+// dz 93, db 7, dx 493, dW 538 us (1.38 to 1.50 PFLOP/s, 0.84 to 0.91 of what a
+// library product reaches in a burst).  One after the other they take 2.0 ms
+// rather than these 1.67: the products draw the power limit.  Pairs of CTAs
+// sharing 256 x 256 tiles, with half the operand traffic, were no faster (551,
+// 515, 550 us).  One token of 4096 x 4096: 6 us (33.6 MB, 5.6 TB/s).
 #include <math_constants.h>
 
 #include "mhc_internal.h"

@@ -28,7 +28,9 @@ from . import _kernels as K
 BLOCK = 256  # elements that share a scale; a tensor's state starts at a multiple of it
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 _M32 = 0xFFFFFFFF
-_contiguous, _data_ptr, _grad = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, attrgetter("grad")
+_contiguous, _data_ptr, _numel, _get_device = (
+    torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device)
+_grad, _dtype = attrgetter("grad"), attrgetter("dtype")
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -77,6 +79,8 @@ class _Pack:
         self.off = (ctypes.c_int64 * n)(*offsets)
         # every gradient must lie in memory as its parameter does
         self.plain = all(p.is_contiguous() for p in params)
+        self.strides = [p.stride() for p in params]
+        self.sizes, self.where = sizes, params[0].get_device()
         zeros = lambda k, dt: torch.zeros(max(k, 1), dtype=dt, device=self.device)[:k]  # noqa: E731
         f8, f32 = torch.float8_e4m3fn, torch.float32
         if bits == 8:
@@ -115,6 +119,7 @@ class _Pack:
             missing = any(g is None for g in grads)
             grads = [g if g is None or not g.is_sparse and g.stride() == p.stride()
                      else self._as_param(p, g) for p, g in zip(self.params, grads)]
+        self._check_forms(grads, not missing)
         if missing or self.steps.count(self.steps[0]) != len(self.steps):
             # the parameters of each number of steps in a launch of their own
             by_step: dict[int, list[int]] = {}
@@ -138,6 +143,23 @@ class _Pack:
         p_ptr, g_ptr = array("Q", map(_data_ptr, self.params)), array("Q", map(_data_ptr, grads))
         self._call(group, t, seed, grad_scale, len(grads), p_ptr.buffer_info()[0],
                    g_ptr.buffer_info()[0], self.numel, self.off)
+
+    def _check_forms(self, grads, whole: bool) -> None:
+        """The kernel goes by the sizes, type and device that the state was laid out for;
+        a parameter may have been given other memory since (``p.data = ...``,
+        ``model.half()``).  torch holds a gradient to its parameter's type and device when
+        it is assigned, so of gradients the size alone is looked at."""
+        ps, n = self.params, len(self.params)
+        if list(map(_numel, ps)) != self.sizes or list(map(_dtype, ps)) != [self.dtype] * n or \
+                list(map(_get_device, ps)) != [self.where] * n or \
+                not (all(map(_contiguous, ps)) if self.plain
+                     else [p.stride() for p in ps] == self.strides):
+            raise ValueError("a parameter has another type, device, size or layout than when "
+                             "its optimizer was made")
+        sizes = list(map(_numel, grads)) if whole else \
+            [k if g is None else g.numel() for g, k in zip(grads, self.sizes)]
+        if sizes != self.sizes:
+            raise ValueError("a gradient has another size than its parameter")
 
     @staticmethod
     def _as_param(p, g):

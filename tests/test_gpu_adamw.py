@@ -354,3 +354,24 @@ def test_repeatable_and_captured():
         runs.append([p.detach().clone() for p in params] +
                     [b.view(torch.uint8).clone() for b in opt.state_buffers().values()])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_parameters_given_other_memory():
+    """New memory of the same form is followed; another type or size is refused."""
+    (p,) = _params([(300,)], torch.float32, 1)
+    opt = mhc_b200.AdamW([p], **HYPER)
+    _set_grads([p], 2)
+    opt.step()
+    p.data = p.data.clone()
+    before = p.detach().clone()
+    opt.step()
+    assert not torch.equal(p.detach(), before)
+    p.data = p.data.half()
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="another type"):
+        opt.step()
+    p.grad = None
+    p.data = torch.zeros(200, device=DEV)
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="another type"):
+        opt.step()

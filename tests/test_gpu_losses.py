@@ -356,3 +356,27 @@ def test_captured_in_a_graph():
     want = run()
     for a, b in zip(out, want):
         assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def test_logits_past_32_bits():
+    """70000 rows of 32000: values past 2^31 are read and written where they are."""
+    T, V = 70000, 32000
+    x = torch.zeros(T, V, dtype=torch.bfloat16, device=DEV)
+    y = torch.full((T,), IGN, dtype=torch.int64, device=DEV)
+    for t in (0, 1, T - 1):
+        y[t] = t % V
+        x[t, t % V] = 4.0
+    old, adv = torch.full((T,), -1.0, device=DEV), torch.ones(T, device=DEV)
+    r = mhc_b200.policy_loss_grad(x, y, old, adv, clip_high=1e9)
+    want = 4.0 - torch.log(torch.tensor(V - 1 + torch.e ** 4)).item()
+    lp = r.logprobs[[0, 1, T - 1]]
+    assert (lp - want).abs().max() <= 1e-5 and not r.logprobs[2:T - 1].any()
+    p = torch.softmax(x[T - 1].double(), 0)
+    c = -float((r.logprobs[T - 1].double() + 1).exp()) / 3
+    row = r.dlogits[T - 1].double()
+    want_row = -c * p
+    want_row[(T - 1) % V] += c
+    assert (row - want_row).abs().max() <= 2.0 ** -8 * abs(c)
+    assert torch.equal(r.dlogits[T - 1, 1:5], r.dlogits[0, 1:5]) and not r.dlogits[2:T - 1:997].any()
+    del x, r
+    torch.cuda.empty_cache()
