@@ -12,6 +12,10 @@ source and header together with the compiler flags, compiles that hash into
 the library (``mhc_build_id()``) and writes it beside the library
 (``libmhc_b200.so.id``).  A library whose id differs from the hash of the
 sources next to it is rebuilt, and the ctypes loader refuses to load one.
+
+``_lib/_mhc_host.so`` is a small Python extension (g++, torch's headers) that
+looks over hundreds of tensors in one call; its id also covers the versions of
+Python and torch that it was compiled for.
 """
 
 from __future__ import annotations
@@ -22,6 +26,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -33,6 +38,9 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libmhc_b200.so"
 ID_PATH = LIB_DIR / "libmhc_b200.so.id"
 OBJ_DIR = LIB_DIR / "obj"
+HOST_SRC = SRC_DIR / "mhc_host.cpp"
+HOST_PATH = LIB_DIR / "_mhc_host.so"
+HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
@@ -86,7 +94,50 @@ def is_stale() -> bool:
 
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = True) -> Path:
-    """Compile every csrc/*.cu for sm_100a and link libmhc_b200.so."""
+    """Compile every csrc/*.cu for sm_100a and link libmhc_b200.so; then the
+    Python extension."""
+    build_library(force, jobs, verbose)
+    build_host(force, verbose)
+    return LIB_PATH
+
+
+def host_id() -> str:
+    """sha256 (first 16 hex digits) of the extension's source, its flags and the
+    versions that it is compiled for."""
+    import torch
+
+    h = hashlib.sha256(HOST_SRC.read_bytes())
+    h.update(f"{HOST_FLAGS} {sys.version} {torch.__version__} {torch.version.git_version}".encode())
+    return h.hexdigest()[:16]
+
+
+def build_host(force: bool = False, verbose: bool = True) -> Path:
+    bid = host_id()
+    stamp = HOST_PATH.with_suffix(".so.id")
+    if not force and HOST_PATH.exists() and stamp.exists() and stamp.read_text().strip() == bid:
+        return HOST_PATH
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    include = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+               Path(sysconfig.get_paths()["include"])]
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", *HOST_FLAGS, f"-DMHC_HOST_ID=\"{bid}\"",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-isystem{p}" for p in include), str(HOST_SRC), "-o", str(tmp),
+           f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    if verbose:
+        print("[mhc_b200 build]", " ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {HOST_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST_PATH)
+    stamp.write_text(bid + "\n")
+    return HOST_PATH
+
+
+def build_library(force: bool = False, jobs: int | None = None, verbose: bool = True) -> Path:
     if not force and not is_stale():
         return LIB_PATH
     nvcc = _nvcc()

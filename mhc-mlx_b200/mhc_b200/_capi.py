@@ -162,6 +162,31 @@ def _check_build_id(lib: ctypes.CDLL, path: Path) -> None:
             f"{want}); rebuild it with `python -m mhc_b200._build`.")
 
 
+_host = None
+
+
+def host():
+    """The extension that looks over many tensors in one call, built with the library."""
+    global _host
+    if _host is None:
+        import importlib.util
+
+        from . import _build
+
+        path = _build.HOST_PATH
+        if not path.exists():
+            raise RuntimeError(f"{path.name} not found at {path}; build it with "
+                               "`python -m mhc_b200._build`.")
+        spec = importlib.util.spec_from_file_location("_mhc_host", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        if _build.HOST_SRC.exists() and module.build_id != _build.host_id():
+            raise RuntimeError(f"{path} was built from another source or for another torch; "
+                               "rebuild it with `python -m mhc_b200._build`.")
+        _host = module
+    return _host
+
+
 def exported_symbols() -> list[str]:
     lib = load()
     return [n for n in SIGNATURES if hasattr(lib, n)]

@@ -17,8 +17,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from array import array
-from operator import attrgetter
 
 import torch
 
@@ -28,9 +26,6 @@ from . import _kernels as K
 BLOCK = 256  # elements that share a scale; a tensor's state starts at a multiple of it
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 _M32 = 0xFFFFFFFF
-_contiguous, _data_ptr, _numel, _get_device = (
-    torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device)
-_grad, _dtype = attrgetter("grad"), attrgetter("dtype")
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -80,7 +75,9 @@ class _Pack:
         # every gradient must lie in memory as its parameter does
         self.plain = all(p.is_contiguous() for p in params)
         self.strides = [p.stride() for p in params]
-        self.sizes, self.where = sizes, params[0].get_device()
+        # written by each step's look at the parameters, read by its launch
+        self.p_ptr, self.g_ptr = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)()
+        self.code, self.where = C.dtype_code(self.dtype), params[0].get_device()
         zeros = lambda k, dt: torch.zeros(max(k, 1), dtype=dt, device=self.device)[:k]  # noqa: E731
         f8, f32 = torch.float8_e4m3fn, torch.float32
         if bits == 8:
@@ -109,61 +106,53 @@ class _Pack:
         return {k: self.view(k, self.params[i], self.offsets[i]) for k in self.buffers}
 
     def launch(self, group, seed: int, grad_scale) -> None:
-        grads = list(map(_grad, self.params))
-        missing = False
-        try:
-            plain = self.plain and all(map(_contiguous, grads))
-        except TypeError:  # a None: a parameter without a gradient
-            plain = False
-        if not plain:
-            missing = any(g is None for g in grads)
-            grads = [g if g is None or not g.is_sparse and g.stride() == p.stride()
-                     else self._as_param(p, g) for p, g in zip(self.params, grads)]
-        self._check_forms(grads, not missing)
-        if missing or self.steps.count(self.steps[0]) != len(self.steps):
-            # the parameters of each number of steps in a launch of their own
-            by_step: dict[int, list[int]] = {}
-            for i, g in enumerate(grads):
-                if g is not None:
-                    by_step.setdefault(self.steps[i], []).append(i)
-            for t, which in by_step.items():
-                n = len(which)
-                self._call(group, t + 1, seed, grad_scale, n,
-                           (ctypes.c_uint64 * n)(*(self.params[i].data_ptr() for i in which)),
-                           (ctypes.c_uint64 * n)(*(grads[i].data_ptr() for i in which)),
-                           (ctypes.c_int64 * n)(*(self.numel[i] for i in which)),
-                           (ctypes.c_int64 * n)(*(self.offsets[i] for i in which)))
-                for i in which:
-                    self.steps[i] = t + 1
+        n = len(self.params)
+        at = ctypes.addressof
+        if self.plain and C.host().gather(self.params, at(self.numel), self.code, self.where,
+                                          at(self.p_ptr), at(self.g_ptr)) \
+                and self.steps.count(self.steps[0]) == n:
+            t = self.steps[0] + 1
+            self.steps = [t] * n
+            if self.total:
+                self._call(group, t, seed, grad_scale, n, self.p_ptr, self.g_ptr, self.numel,
+                           self.off)
             return
-        t = self.steps[0] + 1
-        self.steps = [t] * len(grads)
-        if self.total == 0:
-            return
-        p_ptr, g_ptr = array("Q", map(_data_ptr, self.params)), array("Q", map(_data_ptr, grads))
-        self._call(group, t, seed, grad_scale, len(grads), p_ptr.buffer_info()[0],
-                   g_ptr.buffer_info()[0], self.numel, self.off)
+        # parameters without a gradient, gradients in another order, or an error
+        self._check_forms()
+        grads = [p.grad for p in self.params]
+        grads = [g if g is None or g.layout == torch.strided and not g.is_neg() and
+                 g.stride() == p.stride() else self._as_param(p, g)
+                 for p, g in zip(self.params, grads)]
+        by_step: dict[int, list[int]] = {}  # those of each number of steps in a launch of their own
+        for i, g in enumerate(grads):
+            if g is not None:
+                by_step.setdefault(self.steps[i], []).append(i)
+        for t, which in by_step.items():
+            k = len(which)
+            self._call(group, t + 1, seed, grad_scale, k,
+                       (ctypes.c_uint64 * k)(*(self.params[i].data_ptr() for i in which)),
+                       (ctypes.c_uint64 * k)(*(grads[i].data_ptr() for i in which)),
+                       (ctypes.c_int64 * k)(*(self.numel[i] for i in which)),
+                       (ctypes.c_int64 * k)(*(self.offsets[i] for i in which)))
+            for i in which:
+                self.steps[i] = t + 1
 
-    def _check_forms(self, grads, whole: bool) -> None:
-        """The kernel goes by the sizes, type and device that the state was laid out for;
-        a parameter may have been given other memory since (``p.data = ...``,
-        ``model.half()``).  torch holds a gradient to its parameter's type and device when
-        it is assigned, so of gradients the size alone is looked at."""
-        ps, n = self.params, len(self.params)
-        if list(map(_numel, ps)) != self.sizes or list(map(_dtype, ps)) != [self.dtype] * n or \
-                list(map(_get_device, ps)) != [self.where] * n or \
-                not (all(map(_contiguous, ps)) if self.plain
-                     else [p.stride() for p in ps] == self.strides):
-            raise ValueError("a parameter has another type, device, size or layout than when "
-                             "its optimizer was made")
-        sizes = list(map(_numel, grads)) if whole else \
-            [k if g is None else g.numel() for g, k in zip(grads, self.sizes)]
-        if sizes != self.sizes:
-            raise ValueError("a gradient has another size than its parameter")
+    def _check_forms(self) -> None:
+        """The kernel goes by the sizes, type, device and layout that the state was made
+        for; a parameter may have been given other memory since (``p.data = ...``,
+        ``model.half()``)."""
+        for p, size, strides in zip(self.params, self.numel, self.strides):
+            laid_out = p.is_contiguous() if self.plain else p.stride() == strides
+            if not laid_out or (p.numel(), p.dtype, p.device) != (size, self.dtype, self.device):
+                raise ValueError("a parameter has another type, device, size or layout than when "
+                                 "its optimizer was made")
+            g = p.grad
+            if g is not None and (g.shape, g.dtype, g.device) != (p.shape, p.dtype, p.device):
+                raise ValueError("a gradient does not fit its parameter")
 
     @staticmethod
     def _as_param(p, g):
-        if g.is_sparse:
+        if g.layout != torch.strided:
             raise ValueError("AdamW does not take sparse gradients")
         return torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
 
@@ -280,6 +269,13 @@ class AdamW(torch.optim.Optimizer):
                 pack.steps = [int(step)] * len(pack.params)
 
     # ----------------------------------------------------- save and resume --
+    def __getstate__(self) -> dict:  # copies and pickles: all but the views, made on use
+        return {k: v for k, v in self.__dict__.items() if k != "state"}
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        self.state = _States(self)
+
     def _where(self) -> dict:
         return {p: (pack, i) for packs in self._packs for pack in packs
                 for i, p in enumerate(pack.params)}

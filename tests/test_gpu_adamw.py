@@ -375,3 +375,20 @@ def test_parameters_given_other_memory():
     p.grad = torch.ones_like(p)
     with pytest.raises(ValueError, match="another type"):
         opt.step()
+
+
+def test_copied_optimizer_steps_its_own_parameters():
+    import copy
+
+    (p,) = _params([(300,)], torch.float32, 1)
+    opt = mhc_b200.AdamW([p], **HYPER)
+    _set_grads([p], 2)
+    opt.step()
+    twin = copy.deepcopy(opt)
+    (q,) = twin.param_groups[0]["params"]
+    q.grad = p.grad.clone()
+    before = p.detach().clone()
+    twin.step()
+    assert torch.equal(p.detach(), before) and not torch.equal(q.detach(), before)
+    opt.step()
+    assert torch.equal(p.detach(), q.detach())

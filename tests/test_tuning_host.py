@@ -150,3 +150,26 @@ def test_linear_entry_points_check_their_arguments():
     with pytest.raises(ValueError, match="z"):
         _capi.call("mhc_linear_bwd", 256, 64, None, 0, 256, 64, 256, 64, 2, 1, 256, 64, None, 0, None,
                    100, 64, 64, None, 0, None)
+
+
+def test_host_extension():
+    """It is built from the source beside it, takes CUDA tensors only, and refuses bad calls."""
+    import ctypes
+
+    from mhc_b200 import _build
+
+    host = _capi.host()
+    assert host.build_id == _build.host_id()
+    p = torch.nn.Parameter(torch.zeros(4))
+    numel, out = (ctypes.c_int64 * 1)(4), (ctypes.c_uint64 * 1)(7)
+    at = ctypes.addressof
+    assert host.gather([p], at(numel), 0, 0, at(out), at(out)) is False and out[0] == 7
+    assert host.gather([3], at(numel), 0, 0, at(out), at(out)) is False
+    assert host.gather([], at(numel), 0, 0, at(out), at(out)) is True
+    for bad in (((p,), at(numel), 0, 0, at(out), at(out)), ([p], at(numel), 0, 0, at(out))):
+        with pytest.raises(TypeError):
+            host.gather(*bad)
+    for bad in (([p], 0, 0, 0, at(out), at(out)), ([p], at(numel), 9, 0, at(out), at(out)),
+                ([p], at(numel), 0, -1, at(out), at(out))):
+        with pytest.raises(ValueError):
+            host.gather(*bad)
