@@ -14,8 +14,8 @@ the library (``mhc_build_id()``) and writes it beside the library
 sources next to it is rebuilt, and the ctypes loader refuses to load one.
 
 ``_lib/_mhc_host.so`` is a small Python extension (g++, torch's headers) that
-looks over hundreds of tensors in one call; its id also covers the versions of
-Python and torch that it was compiled for.
+does the host's part of the linear layer and of an optimizer step; its id also
+covers the versions of Python and torch that it was compiled for.
 """
 
 from __future__ import annotations
@@ -106,7 +106,7 @@ def host_id() -> str:
     versions that it is compiled for."""
     import torch
 
-    h = hashlib.sha256(HOST_SRC.read_bytes())
+    h = hashlib.sha256(HOST_SRC.read_bytes() + (INCLUDE_DIR / "mhc_b200.h").read_bytes())
     h.update(f"{HOST_FLAGS} {sys.version} {torch.__version__} {torch.version.git_version}".encode())
     return h.hexdigest()[:16]
 
@@ -120,13 +120,14 @@ def build_host(force: bool = False, verbose: bool = True) -> Path:
 
     torch_dir = Path(torch.__file__).resolve().parent
     include = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
-               Path(sysconfig.get_paths()["include"])]
+               Path(sysconfig.get_paths()["include"]), INCLUDE_DIR,
+               Path(_nvcc()).resolve().parent.parent / "include"]
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = HOST_PATH.with_suffix(".so.tmp")
     cmd = [shutil.which("g++") or "g++", *HOST_FLAGS, f"-DMHC_HOST_ID=\"{bid}\"",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            *(f"-isystem{p}" for p in include), str(HOST_SRC), "-o", str(tmp),
-           f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+           f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     if verbose:
         print("[mhc_b200 build]", " ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)

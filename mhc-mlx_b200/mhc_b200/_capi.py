@@ -166,7 +166,7 @@ _host = None
 
 
 def host():
-    """The extension that looks over many tensors in one call, built with the library."""
+    """The extension with the host's part of some calls, built with the library."""
     global _host
     if _host is None:
         import importlib.util
@@ -183,6 +183,10 @@ def host():
         if _build.HOST_SRC.exists() and module.build_id != _build.host_id():
             raise RuntimeError(f"{path} was built from another source or for another torch; "
                                "rebuild it with `python -m mhc_b200._build`.")
+        lib = load()
+        module.bind(*(ctypes.cast(getattr(lib, n), _P).value for n in (
+            "mhc_linear_fwd_workspace_bytes", "mhc_linear_fwd", "mhc_linear_bwd_workspace_bytes",
+            "mhc_linear_bwd", "mhc_last_error")))
         _host = module
     return _host
 

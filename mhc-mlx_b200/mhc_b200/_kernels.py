@@ -595,62 +595,3 @@ def adamw_step(dev: torch.device, count: int, params, grads, numel, offsets, dty
               C.dtype_code(dtype), bits, C.ptr(exp_avg), C.ptr(exp_avg_scale), C.ptr(exp_avg_sq),
               C.ptr(exp_avg_sq_scale), C.ptr(master), b1, omb1, b2, omb2, decay, step_size,
               inv_sqrt_correction, eps, C.ptr(scale), key, C.stream_of(exp_avg))
-
-
-# ----------------------------------------------------------------- linear --
-def _rows(t: torch.Tensor):
-    """(t, distance between its rows) of [..., C] taken as [rows, C]: in place where
-    its strides allow, else a copy."""
-    if t.is_contiguous():
-        return t, t.shape[-1]
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        t = t.contiguous()
-    t = t.reshape(-1, t.shape[-1])
-    if t.shape[0] <= 1:
-        return t, t.shape[1]
-    if t.stride(0) < t.shape[1]:  # rows that overlap (an expanded tensor)
-        t = t.contiguous()
-    return t, t.stride(0)
-
-
-def linear_fwd(x, weight, bias, residual, act: int, keep_z: bool):
-    """(y, z): z is the pre-activation, rows padded to a multiple of 8, or None."""
-    dev = C.require_cuda(x, weight, bias, residual)
-    N, Kc = weight.shape
-    with _on(dev):
-        M = x.numel() // Kc
-        (x2, ldx), (w2, ldw) = _rows(x), _rows(weight)
-        r2, ldr = (None, 0) if residual is None else _rows(residual)
-        b1 = None if bias is None else _c(bias)
-        y = x.new_empty(*x.shape[:-1], N)
-        ldz = (N + 7) // 8 * 8
-        z = x.new_empty(M, ldz) if keep_z else None
-        px, pw = x2.data_ptr(), w2.data_ptr()
-        nb, ws = 0, None
-        if (px | pw | 2 * ldx | 2 * ldw) & 15:  # rows that need padded copies
-            nb = int(C.query("mhc_linear_fwd_workspace_bytes", px, ldx, pw, ldw, M, N, Kc))
-            ws = _ws(nb, dev) if nb else None
-        _call("mhc_linear_fwd", x2, px, ldx, pw, ldw, C.ptr(b1), C.ptr(r2), ldr,
-              C.dtype_code(x.dtype), act, C.ptr(z), ldz, y.data_ptr(), N, M, N, Kc, C.ptr(ws), nb,
-              C.stream_of(x2))
-    return y, z
-
-
-def linear_bwd(dy, z, x, weight, act: int, want_dx: bool, want_dw: bool, want_db: bool):
-    """(dx, dweight, dbias), None where not wanted."""
-    dev = C.require_cuda(dy, x, weight)
-    N, Kc = weight.shape
-    with _on(dev):
-        M = x.numel() // Kc
-        (d2, ldd), (x2, ldx), (w2, ldw) = _rows(dy), _rows(x), _rows(weight)
-        dx = x.new_empty(x.shape) if want_dx else None
-        dw = x.new_empty(N, Kc) if want_dw else None
-        db = x.new_empty(N) if want_db else None
-        pd, px, pw = d2.data_ptr(), x2.data_ptr(), w2.data_ptr()
-        nb = int(C.query("mhc_linear_bwd_workspace_bytes", pd, ldd, px, ldx, pw, ldw, act, want_dx,
-                         want_dw, want_db, M, N, Kc))
-        ws = _ws(nb, dev) if nb else None
-        _call("mhc_linear_bwd", x2, pd, ldd, C.ptr(z), 0 if z is None else z.shape[1], px, ldx, pw,
-              ldw, C.dtype_code(x.dtype), act, C.ptr(dx), Kc, C.ptr(dw), Kc, C.ptr(db), M, N, Kc,
-              C.ptr(ws), nb, C.stream_of(x2))
-    return dx, dw, db

@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import _kernels as K
+from . import _capi as C
 
 ACTIVATIONS = ("none", "relu", "silu", "gelu")  # gelu: with the error function
 _HALF = (torch.float16, torch.bfloat16)
@@ -42,26 +42,6 @@ def _check(x, weight, bias, residual, activation) -> int:
     return ACTIVATIONS.index(activation)
 
 
-class _LinearFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act):
-        wants = any(ctx.needs_input_grad[:3])
-        y, z = K.linear_fwd(x, weight, bias, residual, act, keep_z=wants and act != 0)
-        ctx.save_for_backward(x, weight, *(() if z is None else (z,)))
-        ctx.act, ctx.has_bias = act, bias is not None
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, *z = ctx.saved_tensors
-        wx, ww, wb, wr, _ = ctx.needs_input_grad
-        dx = dw = db = None
-        if wx or ww or wb:
-            dx, dw, db = K.linear_bwd(dy, z[0] if z else None, x, weight, ctx.act, wx, ww, wb)
-        return dx, dw, db, dy if wr else None, None
-
-
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                residual: torch.Tensor | None = None, activation: str = "none") -> torch.Tensor:
     """act(x W^T + bias) + residual.
@@ -72,11 +52,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     type; with an activation the pre-activation (kept for the backward) and its
     gradient (an operand of the products) are rounded to the type too."""
     act = _check(x, weight, bias, residual, activation)
-    if not torch.is_grad_enabled() or not any(
-            t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        # a decoding step: nothing to record
-        return K.linear_fwd(x, weight, bias, residual, act, keep_z=False)[0]
-    return _LinearFn.apply(x, weight, bias, residual, act)
+    return C.host().linear(x, weight, bias, residual, act)
 
 
 class FusedLinear(nn.Linear):

@@ -233,3 +233,31 @@ def test_module_in_a_rewired_model():
 
 def test_mhc_b200_exports():
     assert mhc_b200.FusedLinear is FusedLinear
+
+
+def test_differentiated_once_only():
+    x, w, _, _, dy = _make(20, 48, 64, torch.bfloat16, 1)
+    x.requires_grad_(), w.requires_grad_()
+    plain = torch.autograd.grad(linear_act(x, w, activation="silu"), [x, w], dy)
+    kept = torch.autograd.grad(linear_act(x, w, activation="silu"), [x, w], dy, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, kept))
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(kept[0].sum(), w)
+
+
+def test_only_what_is_asked_for():
+    """Each operand's gradient by itself is the one that it has among the others."""
+    *ts, dy = _make(40, 56, 72, torch.float16, 2)
+    f = lambda t: linear_act(t[0], t[1], t[2], residual=t[3], activation="relu")  # noqa: E731
+    every = [t.clone().requires_grad_() for t in ts]
+    want = torch.autograd.grad(f(every), every, dy)
+    for i in range(4):
+        one = [t.clone().requires_grad_(i == k) for k, t in enumerate(ts)]
+        assert torch.equal(torch.autograd.grad(f(one), one[i], dy)[0], want[i])
+        assert torch.equal(torch.autograd.grad(f(every), every[i], dy)[0], want[i])
+    x = ts[0].clone().requires_grad_()
+    y = linear_act(x, ts[1])
+    with torch.no_grad():
+        x.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
