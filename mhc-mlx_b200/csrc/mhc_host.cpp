@@ -1,4 +1,4 @@
-// The parts of two operators that run on the host for every call and took longer
+// The parts of operators that run on the host for every call and took longer
 // from Python than their kernels do.
 //
 //   gather   what an optimizer step asks of hundreds of tensors: 512 parameters'
@@ -7,7 +7,11 @@
 //   linear   the linear layer over the C ABI, and its place in autograd: the
 //            engine calls a backward that is written in Python with the
 //            interpreter's lock, on a thread of its own.
+//   token_logprobs, logits_grad, preference, policy   the losses' outputs,
+//            workspaces and calls.
 #include <Python.h>
+
+#include <cstring>
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -33,6 +37,11 @@ struct Library {
   decltype(&mhc_linear_fwd) fwd;
   decltype(&mhc_linear_bwd_workspace_bytes) bwd_bytes;
   decltype(&mhc_linear_bwd) bwd;
+  decltype(&mhc_token_logprobs) token_logprobs;
+  decltype(&mhc_logits_grad) logits_grad;
+  decltype(&mhc_preference_loss) preference;
+  decltype(&mhc_policy_workspace_bytes) policy_bytes;
+  decltype(&mhc_policy_loss) policy;
   decltype(&mhc_last_error) last_error;
 } lib = {};
 
@@ -48,6 +57,58 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor workspace(size_t bytes, const Tensor& like) {
   if (bytes == 0) return {};
   return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+}
+
+// All on x's device, which is a GPU; undefined ones do not count.
+void require_cuda(const Tensor& x, std::initializer_list<const Tensor*> others) {
+  TORCH_CHECK(lib.fwd != nullptr, "the library is not loaded");
+  const auto one = [&](const Tensor& t) {
+    if (!t.defined()) return;
+    TORCH_CHECK(t.is_cuda(), "mhc_b200 runs only on CUDA tensors (sm_100a kernels); got a tensor on ",
+                t.device(), ".  There is no CPU fallback.");
+    TORCH_CHECK_VALUE(t.device() == x.device(), "tensors on different devices: ", x.device(), " and ",
+                      t.device());
+  };
+  one(x);
+  for (const Tensor* t : others) one(*t);
+}
+
+// A call's arguments.
+struct Args {
+  const char* fn;
+  PyObject* const* v;
+  Args(const char* fn_, PyObject* const* v_, Py_ssize_t n, Py_ssize_t want) : fn(fn_), v(v_) {
+    TORCH_CHECK_TYPE(n == want, fn, ": ", want, " arguments are expected, got ", n);
+  }
+  const Tensor& tensor(int i) const {
+    TORCH_CHECK_TYPE(THPVariable_Check(v[i]), fn, ": argument ", i, " must be a tensor");
+    return THPVariable_Unpack(v[i]);
+  }
+  Tensor maybe(int i) const { return v[i] == Py_None ? Tensor() : tensor(i); }
+  int64_t integer(int i) const {
+    const long long k = PyLong_AsLongLong(v[i]);
+    if (k == -1 && PyErr_Occurred()) throw python_error();
+    return k;
+  }
+  float number(int i) const {
+    const double d = PyFloat_AsDouble(v[i]);
+    if (d == -1.0 && PyErr_Occurred()) throw python_error();
+    return (float)d;
+  }
+};
+PyObject* tuple_of(std::initializer_list<Tensor> ts) {
+  PyObject* out = PyTuple_New((Py_ssize_t)ts.size());
+  if (!out) throw python_error();
+  Py_ssize_t i = 0;
+  for (const Tensor& t : ts) {
+    PyObject* o = t.defined() ? THPVariable_Wrap(t) : Py_NewRef(Py_None);
+    if (!o) {
+      Py_DECREF(out);
+      throw python_error();
+    }
+    PyTuple_SET_ITEM(out, i++, o);
+  }
+  return out;
 }
 
 // ----------------------------------------------------------- linear layer --
@@ -146,49 +207,200 @@ struct Linear : torch::autograd::Function<Linear> {
 // Shapes and types have been checked.
 PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(nargs == 5 && THPVariable_Check(args[0]) && THPVariable_Check(args[1]) &&
-                       (args[2] == Py_None || THPVariable_Check(args[2])) &&
-                       (args[3] == Py_None || THPVariable_Check(args[3])) && PyLong_Check(args[4]),
-                   "linear(x, weight, bias, residual, act): tensors and an int are expected");
-  const Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
-  std::optional<Tensor> bias, residual;
-  if (args[2] != Py_None) bias = THPVariable_Unpack(args[2]);
-  if (args[3] != Py_None) residual = THPVariable_Unpack(args[3]);
-  const long act = PyLong_AsLong(args[4]);
-  if (PyErr_Occurred()) return nullptr;
-  TORCH_CHECK(lib.fwd != nullptr, "the library is not loaded");
-  for (const Tensor* t : {&x, &w, bias ? &*bias : &x, residual ? &*residual : &x}) {
-    TORCH_CHECK(t->is_cuda(), "mhc_b200 runs only on CUDA tensors (sm_100a kernels); got a tensor on ",
-                t->device(), ".  There is no CPU fallback.");
-    TORCH_CHECK_VALUE(t->device() == x.device(), "tensors on different devices: ", x.device(), " and ",
-                      t->device());
-  }
+  const Args in("linear", args, nargs, 5);
+  const Tensor &x = in.tensor(0), &w = in.tensor(1);
+  const Tensor b = in.maybe(2), r = in.maybe(3);
+  const int64_t act = in.integer(4);
+  require_cuda(x, {&w, &b, &r});
   Tensor y;
   {
     const pybind11::gil_scoped_release unlocked;
-    const auto needs = [](const std::optional<Tensor>& t) { return t && t->requires_grad(); };
-    const bool wants = x.requires_grad() || w.requires_grad() || needs(bias);
-    if (at::GradMode::is_enabled() && (wants || needs(residual)))
-      y = Linear::apply(x, w, bias, residual, (int64_t)act, wants);
+    const auto needs = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
+    const auto given = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
+    const bool wants = needs(x) || needs(w) || needs(b);
+    if (at::GradMode::is_enabled() && (wants || needs(r)))
+      y = Linear::apply(x, w, given(b), given(r), act, wants);
     else  // a decoding step: nothing to record
-      y = linear_fwd(x, w, bias.value_or(Tensor()), residual.value_or(Tensor()), (int)act, false, nullptr);
+      y = linear_fwd(x, w, b, r, (int)act, false, nullptr);
   }
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of the entry points above, in their order)
+// ----------------------------------------------------------------- losses --
+// Logits [T, V] or [B, S, V] and their targets as the C ABI takes them: rows are
+// read in place where the last axis is contiguous, else copied.
+struct LogitRows {
+  Tensor logits, targets;
+  int64_t rows, per, batch_stride = 0, row_stride, V, ignore;
+  int dtype;
+  LogitRows(const Tensor& x, const Tensor& y, int64_t ignore_) : ignore(ignore_) {
+    V = x.size(-1);
+    logits = x.resolve_neg();
+    if (logits.stride(-1) != 1 && V > 1) logits = logits.contiguous();
+    targets = y.contiguous();
+    rows = targets.numel();
+    per = rows;
+    row_stride = logits.stride(-2);
+    if (logits.dim() == 3) {
+      per = logits.size(1);
+      batch_stride = logits.stride(0);
+    }
+    if (per < 1) per = 1;
+    dtype = logits.scalar_type() == at::kFloat ? MHC_F32
+            : logits.scalar_type() == at::kHalf ? MHC_F16
+                                                : MHC_BF16;
+  }
+  Tensor floats(at::IntArrayRef shape) const {
+    return at::empty(shape, logits.options().dtype(at::kFloat));
+  }
+  // as logits, contiguous
+  Tensor gradient() const { return at::empty(logits.sizes(), logits.options()); }
+};
+Tensor f32(const Tensor& t) {
+  return t.defined() ? t.to(at::kFloat).resolve_neg().contiguous() : t;
+}
+float* at_float(const Tensor& t, int64_t i = 0) {
+  return t.defined() ? t.data_ptr<float>() + i : nullptr;
+}
+
+// token_logprobs(logits, targets, ignore) -> (logp, stats [4 rows])
+PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const Args in("token_logprobs", args, nargs, 3);
+  const Tensor &x = in.tensor(0), &y = in.tensor(1);
+  const int64_t ignore = in.integer(2);
+  require_cuda(x, {&y});
+  Tensor logp, stats;
+  {
+    const pybind11::gil_scoped_release unlocked;
+    const at::AutoGradMode off(false);
+    const c10::cuda::CUDAGuard on(x.device());
+    const LogitRows r(x, y, ignore);
+    logp = r.floats(y.sizes());
+    stats = r.floats({4 * r.rows});
+    check(lib.token_logprobs(ptr(r.logits), r.dtype, r.rows, r.per, r.batch_stride, r.row_stride, r.V,
+                             r.targets.data_ptr<int64_t>(), r.ignore, at_float(logp), at_float(stats),
+                             stream_of(x)),
+          "mhc_token_logprobs");
+  }
+  return tuple_of({logp, stats});
+  END_HANDLE_TH_ERRORS
+}
+
+// logits_grad(logits, targets, ignore, stats, coef or None, scale or None, ready or None)
+//   -> coef * scale * (one-hot - softmax)
+// coef None: it follows the stats, as a loss leaves them.  scale: a device scalar.
+// ready: that gradient for a scale of 1, returned and overwritten unless the scale is 1.
+PyObject* logits_grad(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const Args in("logits_grad", args, nargs, 7);
+  const Tensor &x = in.tensor(0), &y = in.tensor(1), &stats = in.tensor(3);
+  const Tensor coef = in.maybe(4), scale = in.maybe(5), ready = in.maybe(6);
+  const int64_t ignore = in.integer(2);
+  require_cuda(x, {&y, &stats, &coef, &scale, &ready});
+  Tensor out;
+  {
+    const pybind11::gil_scoped_release unlocked;
+    const at::AutoGradMode off(false);
+    const c10::cuda::CUDAGuard on(x.device());
+    const LogitRows r(x, y, ignore);
+    const Tensor c = f32(coef), k = f32(scale);
+    out = ready.defined() ? ready : r.gradient();
+    check(lib.logits_grad(ptr(r.logits), r.dtype, r.rows, r.per, r.batch_stride, r.row_stride, r.V,
+                          r.targets.data_ptr<int64_t>(), r.ignore, at_float(stats),
+                          c.defined() ? at_float(c) : at_float(stats, 4 * r.rows), 1.0f, at_float(k),
+                          ready.defined(), ptr(out), stream_of(x)),
+          "mhc_logits_grad");
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// preference(logits, targets, ignore, ref, cu_seqlens or None, pairs, beta, smoothing,
+//            inverse denominator, grad_scale, want_grad)
+//   -> (loss, logp, margins, dlogits or None, stats and coef [5 rows])
+PyObject* preference(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const Args in("preference", args, nargs, 11);
+  const Tensor &x = in.tensor(0), &y = in.tensor(1), &ref = in.tensor(3);
+  const Tensor cu = in.maybe(4);
+  const int64_t ignore = in.integer(2), pairs = in.integer(5), want = in.integer(10);
+  const float beta = in.number(6), smoothing = in.number(7), inv_d = in.number(8), scale = in.number(9);
+  require_cuda(x, {&y, &ref, &cu});
+  Tensor loss, logp, margins, dlogits, records;
+  {
+    const pybind11::gil_scoped_release unlocked;
+    const at::AutoGradMode off(false);
+    const c10::cuda::CUDAGuard on(x.device());
+    const LogitRows r(x, y, ignore);
+    const Tensor f = f32(ref), c = cu.defined() ? cu.contiguous() : cu;
+    loss = r.floats({});
+    logp = r.floats(y.sizes());
+    margins = r.floats({pairs});
+    records = r.floats({5 * r.rows});
+    if (want) dlogits = r.gradient();
+    check(lib.preference(ptr(r.logits), r.dtype, r.rows, r.per, r.batch_stride, r.row_stride, r.V,
+                         r.targets.data_ptr<int64_t>(), r.ignore, ptr(c),
+                         c.defined() && c.scalar_type() == at::kLong, c.defined() ? 0 : r.logits.size(1),
+                         pairs, at_float(f), beta, smoothing, inv_d, scale, at_float(logp),
+                         at_float(records), at_float(records, 4 * r.rows), at_float(margins),
+                         at_float(loss), ptr(dlogits), stream_of(x)),
+          "mhc_preference_loss");
+  }
+  return tuple_of({loss, logp, margins, dlogits, records});
+  END_HANDLE_TH_ERRORS
+}
+
+// policy(logits, targets, ignore, old, advantages, ref or None, clip_low, clip_high, kl_coef,
+//        inverse denominator or 0, grad_scale, want_grad)
+//   -> (loss, logp, kl, dlogits or None, stats and coef [5 rows])
+PyObject* policy(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const Args in("policy", args, nargs, 12);
+  const Tensor &x = in.tensor(0), &y = in.tensor(1), &old = in.tensor(3), &adv = in.tensor(4);
+  const Tensor ref = in.maybe(5);
+  const int64_t ignore = in.integer(2), want = in.integer(11);
+  const float lo = in.number(6), hi = in.number(7), kl_coef = in.number(8), inv_d = in.number(9),
+              scale = in.number(10);
+  require_cuda(x, {&y, &old, &adv, &ref});
+  Tensor loss, logp, kl, dlogits, records;
+  {
+    const pybind11::gil_scoped_release unlocked;
+    const at::AutoGradMode off(false);
+    const c10::cuda::CUDAGuard on(x.device());
+    const LogitRows r(x, y, ignore);
+    const Tensor o = f32(old), a = f32(adv), f = f32(ref);
+    loss = r.floats({});
+    kl = r.floats({});
+    logp = r.floats(y.sizes());
+    records = r.floats({5 * r.rows});
+    if (want) dlogits = r.gradient();
+    const size_t bytes = lib.policy_bytes();
+    const Tensor ws = workspace(bytes, x);
+    check(lib.policy(ptr(r.logits), r.dtype, r.rows, r.per, r.batch_stride, r.row_stride, r.V,
+                     r.targets.data_ptr<int64_t>(), r.ignore, at_float(o), at_float(a), at_float(f), lo,
+                     hi, kl_coef, inv_d, scale, at_float(logp), at_float(records),
+                     at_float(records, 4 * r.rows), at_float(loss), at_float(kl), ptr(dlogits), ptr(ws),
+                     bytes, stream_of(x)),
+          "mhc_policy_loss");
+  }
+  return tuple_of({loss, logp, kl, dlogits, records});
+  END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses of the entry points of Library, in their order)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  void* p[5];
-  if (nargs != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind: five addresses are expected");
+  constexpr int n = sizeof(Library) / sizeof(void*);
+  void* p[n];
+  if (nargs != n) {
+    PyErr_Format(PyExc_TypeError, "bind: %d addresses are expected", n);
     return nullptr;
   }
-  for (int i = 0; i < 5; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
+  for (int i = 0; i < n; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
   if (PyErr_Occurred()) return nullptr;
-  lib = {reinterpret_cast<decltype(lib.fwd_bytes)>(p[0]), reinterpret_cast<decltype(lib.fwd)>(p[1]),
-         reinterpret_cast<decltype(lib.bwd_bytes)>(p[2]), reinterpret_cast<decltype(lib.bwd)>(p[3]),
-         reinterpret_cast<decltype(lib.last_error)>(p[4])};
+  static_assert(sizeof(Library) == sizeof(p), "one address a member");
+  std::memcpy(&lib, p, sizeof(p));
   Py_RETURN_NONE;
 }
 
@@ -253,7 +465,11 @@ PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
 }
 PyMethodDef methods[] = {
-    {"bind", fast(bind), METH_FASTCALL, "bind(five entry points' addresses)"},
+    {"bind", fast(bind), METH_FASTCALL, "bind(the entry points' addresses)"},
+    {"token_logprobs", fast(token_logprobs), METH_FASTCALL, "-> (logp, stats)"},
+    {"logits_grad", fast(logits_grad), METH_FASTCALL, "-> dlogits"},
+    {"preference", fast(preference), METH_FASTCALL, "-> (loss, logp, margins, dlogits, records)"},
+    {"policy", fast(policy), METH_FASTCALL, "-> (loss, logp, kl, dlogits, records)"},
     {"linear", fast(linear), METH_FASTCALL, "linear(x, weight, bias, residual, act) -> Tensor"},
     {"gather", fast(gather), METH_FASTCALL,
      "gather(params, numel, dtype, device, p_out, g_out) -> bool"},

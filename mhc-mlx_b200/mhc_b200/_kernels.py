@@ -481,108 +481,6 @@ def qlinear_transpose_pack(w_packed, in_dims: int):
     return wt
 
 
-# ------------------------------------------------------- losses on logits --
-class LogitRows:
-    """Logits [T, V] or [B, S, V] and their targets as the C ABI takes them:
-    rows read in place when the last axis is contiguous, else a copy."""
-
-    __slots__ = ("logits", "targets", "shape", "rows", "args", "dev")
-
-    def __init__(self, logits: torch.Tensor, targets: torch.Tensor, ignore_index: int):
-        self.dev = C.require_cuda(logits, targets)
-        strides, V = logits.stride(), logits.shape[-1]
-        if strides[-1] != 1 and V > 1:
-            logits = logits.contiguous()
-            strides = logits.stride()
-        self.logits, self.targets = logits, _c(targets)
-        self.shape, self.rows = targets.shape, targets.numel()
-        if len(strides) == 3:
-            per, sb, sr = logits.shape[1], strides[0], strides[1]
-        else:
-            per, sb, sr = self.rows, 0, strides[0]
-        self.args = (logits.data_ptr(), C.dtype_code(logits.dtype), self.rows, max(per, 1), sb, sr,
-                     V, self.targets.data_ptr(), ignore_index)
-
-    def grad_like(self) -> torch.Tensor:
-        return self.logits.new_empty(self.logits.shape)
-
-    def floats(self, *shape) -> torch.Tensor:
-        return torch.empty(*shape, dtype=F32, device=self.dev)
-
-
-def token_logprobs(r: LogitRows):
-    """(logp, stats): fp32 of the targets' shape, and four floats a row for logits_grad."""
-    with _on(r.dev):
-        logp, stats = r.floats(r.shape), r.floats(r.rows, 4)
-        _call("mhc_token_logprobs", r.logits, *r.args, C.ptr(logp), C.ptr(stats),
-              C.stream_of(r.logits))
-    return logp, stats
-
-
-def logits_grad(r: LogitRows, stats, coef, scale=None, ready=None):
-    """coef * scale * (one-hot - softmax); `scale` is a device scalar or None.
-    `ready`, when given, is that gradient for a scale of 1: it is returned,
-    overwritten unless the scale is 1."""
-    C.require_cuda(r.logits, coef, scale)
-    with _on(r.dev):
-        coef = _f32(coef)
-        scale = None if scale is None else _f32(scale)
-        out = r.grad_like() if ready is None else ready
-        _call("mhc_logits_grad", r.logits, *r.args, C.ptr(stats), C.ptr(coef), 1.0, C.ptr(scale),
-              int(ready is not None), C.ptr(out), C.stream_of(r.logits))
-    return out
-
-
-def _row_records(r: LogitRows, like: torch.Tensor):
-    """(stats, coef) of a loss: five floats a row in one buffer."""
-    rows = r.rows
-    both = like.new_empty(5 * rows)
-    return both, both.data_ptr(), both.data_ptr() + 16 * rows
-
-
-def split_records(both: torch.Tensor):
-    """(stats [rows, 4], coef [rows]) of a loss's records."""
-    rows = both.numel() // 5
-    return both[:4 * rows].view(rows, 4), both[4 * rows:]
-
-
-def preference_loss(r: LogitRows, ref, cu, pairs: int, beta: float, smoothing: float,
-                    inv_d: float, grad_scale: float, want_grad: bool):
-    """(loss, logp, margins, dlogits or None, records)"""
-    C.require_cuda(r.logits, ref, cu)
-    with _on(r.dev):
-        ref = _f32(ref)
-        cu = None if cu is None else _c(cu)
-        uniform = r.logits.shape[1] if cu is None else 0
-        loss, margins, logp = ref.new_empty(()), ref.new_empty(pairs), ref.new_empty(r.shape)
-        both, stats, coef = _row_records(r, ref)
-        dlogits = r.grad_like() if want_grad else None
-        _call("mhc_preference_loss", r.logits, *r.args, C.ptr(cu),
-              int(cu is not None and cu.dtype == torch.int64), uniform, pairs, ref.data_ptr(), beta,
-              smoothing, inv_d, grad_scale, logp.data_ptr(), stats, coef, margins.data_ptr(),
-              loss.data_ptr(), C.ptr(dlogits), C.stream_of(r.logits))
-    return loss, logp, margins, dlogits, both
-
-
-def policy_loss(r: LogitRows, old, adv, ref, clip_low: float, clip_high: float, kl_coef: float,
-                inv_d: float, grad_scale: float, want_grad: bool):
-    """(loss, logp, kl, dlogits or None, records)"""
-    C.require_cuda(r.logits, old, adv, ref)
-    with _on(r.dev):
-        old, adv = _f32(old), _f32(adv)
-        ref = None if ref is None else _f32(ref)
-        loss, kl, logp = old.new_empty(()), old.new_empty(()), old.new_empty(r.shape)
-        both, stats, coef = _row_records(r, old)
-        dlogits = r.grad_like() if want_grad else None
-        nb = _ws_bytes("mhc_policy_workspace_bytes", r.dev)
-        ws = _ws(nb, r.dev)
-        _call("mhc_policy_loss", r.logits, *r.args, old.data_ptr(), adv.data_ptr(), C.ptr(ref),
-              clip_low, clip_high, kl_coef, inv_d, grad_scale, logp.data_ptr(), stats, coef,
-              loss.data_ptr(), kl.data_ptr(), C.ptr(dlogits), ws.data_ptr(), nb,
-              C.stream_of(r.logits))
-    return loss, logp, kl, dlogits, both
-
-
 # ------------------------------------------------------------------ AdamW --
 def adamw_step(dev: torch.device, count: int, params, grads, numel, offsets, dtype, bits: int,
                exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, master, b1, omb1, b2, omb2,

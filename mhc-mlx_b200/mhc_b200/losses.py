@@ -23,7 +23,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _kernels as K
+from . import _capi as C
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -120,8 +120,7 @@ def _check_policy(logits, targets, old_logprobs, advantages, ref_logprobs, clip_
 class _LogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ignore_index):
-        rows = K.LogitRows(logits, targets, ignore_index)
-        logp, stats = K.token_logprobs(rows)
+        logp, stats = C.host().token_logprobs(logits, targets, ignore_index)
         ctx.save_for_backward(logits, targets, stats)
         ctx.ignore_index = ignore_index
         return logp
@@ -130,8 +129,8 @@ class _LogprobsFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d):
         logits, targets, stats = ctx.saved_tensors
-        rows = K.LogitRows(logits, targets, ctx.ignore_index)
-        return K.logits_grad(rows, stats, d), None, None
+        grad = C.host().logits_grad(logits, targets, ctx.ignore_index, stats, d, None, None)
+        return grad, None, None
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *,
@@ -145,9 +144,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *,
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ref, cu, pairs, beta, smoothing, inv_d, ignore_index):
-        rows = K.LogitRows(logits, targets, ignore_index)
-        loss, logp, margins, _, records = K.preference_loss(
-            rows, ref, cu, pairs, beta, smoothing, inv_d, 1.0, want_grad=False)
+        loss, logp, margins, _, records = C.host().preference(
+            logits, targets, ignore_index, ref, cu, pairs, beta, smoothing, inv_d, 1.0, False)
         ctx.save_for_backward(logits, targets, records)
         ctx.ignore_index = ignore_index
         ctx.mark_non_differentiable(logp, margins)
@@ -157,9 +155,8 @@ class _PreferenceFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d, _logp, _margins):
         logits, targets, records = ctx.saved_tensors
-        rows = K.LogitRows(logits, targets, ctx.ignore_index)
-        stats, coef = K.split_records(records)
-        return (K.logits_grad(rows, stats, coef, scale=d),) + (None,) * 8
+        grad = C.host().logits_grad(logits, targets, ctx.ignore_index, records, None, d, None)
+        return (grad,) + (None,) * 8
 
 
 def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logprobs: torch.Tensor,
@@ -192,11 +189,9 @@ def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor, ref_logpro
     """``preference_loss`` and, in ``dlogits``, grad_scale times its gradient."""
     pairs, inv_d = _check_preference(logits, targets, ref_logprobs, cu_seqlens, label_smoothing,
                                      denominator)
-    rows = K.LogitRows(logits, targets, int(ignore_index))
-    loss, logp, margins, dlogits, _ = K.preference_loss(
-        rows, ref_logprobs, cu_seqlens, pairs, float(beta), float(label_smoothing), inv_d,
-        float(grad_scale), want_grad=True)
-    return PreferenceResult(loss, logp, margins, dlogits)
+    return PreferenceResult(*C.host().preference(
+        logits, targets, int(ignore_index), ref_logprobs, cu_seqlens, pairs, beta, label_smoothing,
+        inv_d, grad_scale, True)[:4])
 
 
 # ----------------------------------------------------------------- policy --
@@ -207,9 +202,9 @@ class _PolicyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, targets, old, adv, ref, lo, hi, kl_coef, inv_d, ignore_index):
-        rows = K.LogitRows(logits, targets, ignore_index)
-        loss, logp, kl, dlogits, records = K.policy_loss(
-            rows, old, adv, ref, lo, hi, kl_coef, inv_d, 1.0, want_grad=ctx.needs_input_grad[0])
+        loss, logp, kl, dlogits, records = C.host().policy(
+            logits, targets, ignore_index, old, adv, ref, lo, hi, kl_coef, inv_d, 1.0,
+            ctx.needs_input_grad[0])
         ctx.save_for_backward(logits, targets, records)
         ctx.ignore_index, ctx.dlogits = ignore_index, dlogits
         ctx.mark_non_differentiable(logp, kl)
@@ -219,11 +214,10 @@ class _PolicyFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d, _logp, _kl):
         logits, targets, records = ctx.saved_tensors
-        rows = K.LogitRows(logits, targets, ctx.ignore_index)
-        stats, coef = K.split_records(records)
         # handed over once: a second backward over a kept graph computes its own
         ready, ctx.dlogits = ctx.dlogits, None
-        return (K.logits_grad(rows, stats, coef, scale=d, ready=ready),) + (None,) * 9
+        grad = C.host().logits_grad(logits, targets, ctx.ignore_index, records, None, d, ready)
+        return (grad,) + (None,) * 9
 
 
 def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch.Tensor,
@@ -254,8 +248,6 @@ def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: 
     """``policy_loss`` and, in ``dlogits``, grad_scale times its gradient."""
     inv_d = _check_policy(logits, targets, old_logprobs, advantages, ref_logprobs, clip_low,
                           clip_high, kl_coef, denominator)
-    rows = K.LogitRows(logits, targets, int(ignore_index))
-    loss, logp, kl, dlogits, _ = K.policy_loss(
-        rows, old_logprobs, advantages, ref_logprobs, float(clip_low), float(clip_high),
-        float(kl_coef), inv_d, float(grad_scale), want_grad=True)
-    return PolicyResult(loss, logp, kl, dlogits)
+    return PolicyResult(*C.host().policy(
+        logits, targets, int(ignore_index), old_logprobs, advantages, ref_logprobs, clip_low,
+        clip_high, kl_coef, inv_d, grad_scale, True)[:4])
