@@ -190,17 +190,60 @@ __device__ __forceinline__ float2 peer_float2(const float2* own, unsigned rank) 
   return v;
 }
 
+// Writes v to `own`'s place in another block of the cluster and counts its 8 bytes
+// on `bar` there.
+__device__ __forceinline__ void send_float2(const float2* own, uint64_t* bar, unsigned rank, float2 v) {
+  unsigned a, b;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(own)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(rank));
+  const uint64_t u = (uint64_t)__float_as_uint(v.x) | (uint64_t)__float_as_uint(v.y) << 32;
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(a), "l"(u),
+               "r"(b)
+               : "memory");
+}
+// As mbar_wait, for what other blocks of the cluster have sent.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, unsigned parity) {
+  for (unsigned k = 0; k < (1u << 22); ++k) {
+    unsigned ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
 // (max, sum) of the whole row, on the first warp of every block that shares it:
 // each warp's, then the warps' by the first, then the blocks' by the first warp
 // of each; the order is fixed.  `k` counts the rows that the block has joined:
 // the slots alternate, so that a slot is written again only after a later
-// row's barrier.  A block of a cluster ends with cluster_arrive();
-// cluster_wait(): a peer may still read its slot.
+// row's barrier.  The blocks of a cluster send their values into each other's
+// slots, counted on an mbarrier there: a cluster barrier would first wait for
+// the gradient's stores of the row before (rows of 50001 fp16 values over two
+// blocks: loss and gradient of 1000 60 us, with the barrier 65).  A block sends for row k + 2 only after it has
+// everyone's values of k + 1, and so after everyone has read those of row k.
 template <int NT>
 struct RowShared {
   float2 warp[2][NT / 32];
-  float2 block[2];
+  float2 block[2][kMaxCluster];
+  uint64_t got[2];
 };
+// Before the first join, by all threads of all blocks of the cluster; they end
+// with cluster_arrive(); cluster_wait().
+template <int NT>
+__device__ __forceinline__ void row_shared_init(RowShared<NT>& sh, int cs) {
+  if (cs == 1) return;
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.got[0], 1);
+    mbar_init(&sh.got[1], 1);
+    mbar_init_fence();
+  }
+  cluster_arrive();
+  cluster_wait();
+}
 template <int NT>
 __device__ __forceinline__ MaxSum row_join(MaxSum v, RowShared<NT>& sh, int cs, unsigned k) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = k & 1;
@@ -210,14 +253,12 @@ __device__ __forceinline__ MaxSum row_join(MaxSum v, RowShared<NT>& sh, int cs, 
   if (warp == 0) {
     const float2 f = lane < NT / 32 ? sh.warp[b][lane] : make_float2(-CUDART_INF_F, 0.f);
     v = warp_join({f.x, f.y});
-    if (cs > 1 && lane == 0) sh.block[b] = make_float2(v.m, v.s);
-  }
-  if (cs > 1) {
-    cluster_arrive();
-    cluster_wait();
-    if (warp == 0) {
-      const float2 g = lane < cs ? peer_float2(&sh.block[b], lane) : make_float2(-CUDART_INF_F, 0.f);
-      v = warp_join({g.x, g.y});
+    if (cs > 1) {
+      if (lane == 0) mbar_arrive_expect_tx(&sh.got[b], 8u * (unsigned)cs);
+      if (lane < cs) send_float2(&sh.block[b][cluster_rank()], &sh.got[b], lane, make_float2(v.m, v.s));
+      const bool got = mbar_wait_cluster(&sh.got[b], (k >> 1) & 1u);
+      const float2 g = lane < cs ? sh.block[b][lane] : make_float2(-CUDART_INF_F, 0.f);
+      v = warp_join({g.x, got ? g.y : CUDART_NAN_F});
     }
   }
   return v;
@@ -569,6 +610,7 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
     mbar_init_fence();
     sm.loss = sm.kl = 0.0;
   }
+  row_shared_init(sm.sh, cs);
   __syncthreads();
   if constexpr (!POLICY) pdl_trigger();
 
@@ -788,6 +830,7 @@ k_long_rows(Rows a, int slice, int cs, float* __restrict__ logp, float4* __restr
     }
     return;
   }
+  row_shared_init(sh, cs);
   const T* x = row_ptr<T>(a, t);
   const float xt = first ? target_logit(x, y, a.V) : 0.f;
   const int64_t lo = (int64_t)rank * slice < a.V ? (int64_t)rank * slice : a.V;
