@@ -127,14 +127,15 @@ __device__ __forceinline__ float max_of(const Vec<T> (&r)[NV]) {
   }
 }
 
-// sum exp(x - m) over NV vectors, m finite.  log2(e) to 48 bits here: with 24
+// sum exp(x - m) over the first n of NV vectors, m finite.  log2(e) to 48 bits here: with 24
 // every term is off the same way (1e-8 of the difference), and a sequence's
 // summed log probabilities keep what their errors have in common.
 template <typename T, int NV>
-__device__ __forceinline__ float sum_of(const Vec<T> (&r)[NV], float m) {
+__device__ __forceinline__ float sum_of(const Vec<T> (&r)[NV], float m, int n) {
   float s0 = 0.f, s1 = 0.f;  // added in pairs
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    if (i >= n) break;
 #pragma unroll
     for (int k = 0; k < Vec<T>::VE / 2; ++k) {
       const float2 f = r[i].pair(k);
@@ -144,6 +145,7 @@ __device__ __forceinline__ float sum_of(const Vec<T> (&r)[NV], float m) {
           : "+f"(s0), "+f"(s1)
           : "f"(e.x), "f"(e.y));
     }
+  }
   return s0 + s1;
 }
 
@@ -222,9 +224,9 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, unsigned parity
 // the slots alternate, so that a slot is written again only after a later
 // row's barrier.  The blocks of a cluster send their values into each other's
 // slots, counted on an mbarrier there: a cluster barrier would first wait for
-// the gradient's stores of the row before (rows of 50001 fp16 values over two
-// blocks: loss and gradient of 1000 60 us, with the barrier 65).  A block sends for row k + 2 only after it has
-// everyone's values of k + 1, and so after everyone has read those of row k.
+// the gradient's stores of the row before (8 % of 1000 rows of 50001 fp16 values,
+// two blocks each).  A block sends for row k + 2 only after it has everyone's
+// values of k + 1, and so after everyone has read those of row k.
 template <int NT>
 struct RowShared {
   float2 warp[2][NT / 32];
@@ -324,12 +326,12 @@ struct Hidden {
   }
 };
 
-// (max, sum) of one thread's NV vectors.
+// (max, sum) of one thread's NV vectors, those from n on -inf throughout.
 template <typename T, int NV>
-__device__ __forceinline__ MaxSum vecs_of(const Vec<T> (&r)[NV]) {
+__device__ __forceinline__ MaxSum vecs_of(const Vec<T> (&r)[NV], int n = NV) {
   const float m = max_of(r);
   // all -inf (or NaN): sum against 0, which gives 0 (or NaN)
-  return {m, sum_of(r, m == -CUDART_INF_F ? 0.f : m)};
+  return {m, sum_of(r, m == -CUDART_INF_F ? 0.f : m, n)};
 }
 
 // --------------------------------------------------------------- the grids --
@@ -467,7 +469,7 @@ struct Grains {
   int count;         // granules
   int skip, last;    // values before the slice in the first, of the slice in the last granule
   int bulk0, bulk1;  // granules [bulk0, bulk1) may be copied whole
-  int ragged;        // the ends need care
+  int head, tail;    // granules that have others' values too, or -1
   __device__ void set(const T* x, int lo, int hi, uintptr_t span0, uintptr_t span1) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(x + lo), b = reinterpret_cast<uintptr_t>(x + hi);
     const uintptr_t a0 = a & ~(uintptr_t)15, b1 = (b + 15) & ~(uintptr_t)15;
@@ -479,7 +481,8 @@ struct Grains {
     bulk0 = a0 < span0 ? 1 : 0;
     bulk1 = b1 > span1 ? count - 1 : count;
     if (bulk1 < bulk0) bulk1 = bulk0;
-    ragged = skip != 0 || last != VE;  // what the copy leaves out is ragged too
+    head = count > 0 && skip != 0 ? 0 : -1;
+    tail = count > 0 && last != VE ? count - 1 : -1;
   }
   // The slice's values in granule j are [from(j), to(j)).
   __device__ __forceinline__ int from(int j) const { return j == 0 ? skip : 0; }
@@ -498,6 +501,18 @@ __device__ __forceinline__ void put(uint4& u, int e, unsigned bits) {
   if (w == 1) u.y = (u.y & ~m) | v;
   if (w == 2) u.z = (u.z & ~m) | v;
   if (w == 3) u.w = (u.w & ~m) | v;
+}
+// The first n values (Below), or those from n on, become -inf.
+template <typename T, bool Below>
+__device__ __forceinline__ void trim(uint4& u, int n) {
+  Vec<T> inf;
+  inf.fill_neg_inf();
+  const auto word = [&](unsigned w, int i) {
+    const int bits = 8 * (int)sizeof(T) * n - 32 * i;  // of this word, below n
+    const unsigned m = bits <= 0 ? 0u : bits >= 32 ? 0xffffffffu : (1u << bits) - 1u;
+    return Below ? (w & ~m) | (inf.u.x & m) : (w & m) | (inf.u.x & ~m);
+  };
+  u = make_uint4(word(u.x, 0), word(u.y, 1), word(u.z, 2), word(u.w, 3));
 }
 template <typename T>
 __device__ __forceinline__ unsigned bits_of(float v) {
@@ -675,7 +690,6 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
     const bool landed = mbar_wait(&sm.full, joined & 1u);
     const Grains<T>& g = sm.grains[joined & 1];  // set again two rows on
     const int count = g.count, skip = g.skip;
-    const bool ragged = g.ragged != 0;
     // the target's granule and its place there
     const int ye = y >= lo && y < hi ? y - lo + skip : -1;
     const int yj = ye >= 0 ? ye / VE : -1;
@@ -693,18 +707,25 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
         r[i].fill_neg_inf();
         if (tid + (i0 + i) * NT < count) r[i].u = slot[tid + (i0 + i) * NT];
       }
-      if (ragged) {  // the ends: other rows' values go, what the copy left out comes
+      if (g.bulk0 != 0 || g.bulk1 != count) {  // value by value, what the copy left out
 #pragma unroll
         for (int i = 0; i < kHold; ++i) {
           const int j = tid + (i0 + i) * NT;
-          if (j < count && (j == 0 || j == count - 1)) {
+          if (j < count && (j < g.bulk0 || j >= g.bulk1)) {
 #pragma unroll 1
             for (int e = 0; e < VE; ++e) {
-              if (e < g.from(j) || e >= g.to(j)) put<T>(r[i].u, e, neg_inf_bits<T>());
-              else if (j < g.bulk0 || j >= g.bulk1) put<T>(r[i].u, e, bits_of<T>(to_f(reinterpret_cast<const T*>(g.at + j)[e])));
+              const bool ours = e >= g.from(j) && e < g.to(j);
+              put<T>(r[i].u, e, ours ? bits_of<T>(to_f(reinterpret_cast<const T*>(g.at + j)[e])) : neg_inf_bits<T>());
             }
           }
         }
+      }
+      // other rows' values at the ends
+      if (g.head == 0 && tid == 0 && i0 == 0) trim<T, true>(r[0].u, skip);
+      if (g.tail >= 0 && g.tail % NT == tid) {
+#pragma unroll
+        for (int i = 0; i < kHold; ++i)
+          if (g.tail == tid + (i0 + i) * NT) trim<T, false>(r[i].u, g.last);
       }
       if (i0 + kHold >= kNV) {
         __syncthreads();
@@ -719,7 +740,8 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
         for (int i = 0; i < kHold; ++i)
           if (yj == tid + (i0 + i) * NT) put<T>(r[i].u, ye % VE, neg_inf_bits<T>());
       }
-      acc = kHold == kNV ? vecs_of(r) : join(acc, vecs_of(r));
+      const int own = (count - tid - i0 * NT + NT - 1) / NT;  // vectors from here on
+      acc = kHold == kNV ? vecs_of(r, own) : join(acc, vecs_of(r, own));
     }
     acc = row_join<NT>(acc, sm.sh, cs, joined);
     ++joined;
@@ -759,19 +781,32 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
       if (out && e.w == 0.f) {
         zero_slice<T, NT>(out, lo, hi);
       } else if (out) {
+        const int count = g.count, skip = g.skip, head = g.head, tail = g.tail;
         T* o = out + (lo - skip) + tid * VE;  // granule j begins at (j - tid) VE from here
-        const bool aligned = (reinterpret_cast<uintptr_t>(o) & 15u) == 0;
-        const bool whole = aligned && !ragged;
+        const auto gradient = [&](const Vec<T>& x, int j) {
+          uint4 v = scaled<T>(x, e.x, e.y);
+          if (mine && j == yj) put<T>(v, ye % VE, bits_of<T>(e.z));
+          return v;
+        };
+        if ((reinterpret_cast<uintptr_t>(o) & 15u) == 0) {
 #pragma unroll
-        for (int i = 0; i < kHold; ++i) {
-          const int j = tid + i * NT;
-          if (j < count) {
-            uint4 v = scaled<T>(r[i], e.x, e.y);
-            if (mine && j == yj) put<T>(v, ye % VE, bits_of<T>(e.z));
-            if (whole || (aligned && g.from(j) == 0 && g.to(j) == VE))
-              __stcs(reinterpret_cast<uint4*>(o) + i * NT, v);
-            else
-              store_values(o + i * NT * VE, v, g.from(j), g.to(j));
+          for (int i = 0; i < kHold; ++i) {
+            const int j = tid + i * NT;
+            if (j < count && j != head && j != tail) __stcs(reinterpret_cast<uint4*>(o) + i * NT, gradient(r[i], j));
+          }
+          if (head == 0 && tid == 0) store_values(o, gradient(r[0], 0), skip, g.to(0));
+          if (tail != head && tail % NT == tid) {
+            Vec<T> x = r[0];
+#pragma unroll
+            for (int i = 1; i < kHold; ++i)
+              if (tail == tid + i * NT) x = r[i];
+            store_values(o + (tail - tid) * VE, gradient(x, tail), 0, g.last);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kHold; ++i) {
+            const int j = tid + i * NT;
+            if (j < count) store_values(o + i * NT * VE, gradient(r[i], j), g.from(j), g.to(j));
           }
         }
       }
