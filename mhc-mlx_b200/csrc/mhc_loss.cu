@@ -135,7 +135,7 @@ __device__ __forceinline__ float sum_of(const Vec<T> (&r)[NV], float m, int n) {
   float s0 = 0.f, s1 = 0.f;  // added in pairs
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (i >= n) break;
+    if (i >= NV / 2 && i >= n) break;  // a branch for each of the first half costs more than it saves
 #pragma unroll
     for (int k = 0; k < Vec<T>::VE / 2; ++k) {
       const float2 f = r[i].pair(k);
@@ -700,7 +700,8 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
     const bool mine = yj >= 0 && yj % NT == tid;  // this thread has the target
     Vec<T> r[kHold];
     MaxSum acc = {-CUDART_INF_F, 0.f};
-#pragma unroll 1
+    // unrolled: a loop over the halves is 10 % slower (8192 x 32000 bf16 sums 99 us, 89)
+#pragma unroll
     for (int i0 = 0; i0 < kNV; i0 += kHold) {
 #pragma unroll
       for (int i = 0; i < kHold; ++i) {
@@ -741,7 +742,7 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
           if (yj == tid + (i0 + i) * NT) put<T>(r[i].u, ye % VE, neg_inf_bits<T>());
       }
       const int own = (count - tid - i0 * NT + NT - 1) / NT;  // vectors from here on
-      acc = kHold == kNV ? vecs_of(r, own) : join(acc, vecs_of(r, own));
+      acc = kHold == kNV ? vecs_of(r, own) : i0 == 0 ? vecs_of(r) : join(acc, vecs_of(r, own));
     }
     acc = row_join<NT>(acc, sm.sh, cs, joined);
     ++joined;
