@@ -101,7 +101,7 @@ SIGNATURES: dict[str, tuple] = {
 _lib = None
 _lock = threading.Lock()
 
-# Number of status-returning C-ABI calls made by this process.  Every such
+# Number of status-returning C-ABI calls made by `call` in this process.  Every such
 # call enqueues kernels; the benchmark uses the count to report launches.
 CALLS = 0
 

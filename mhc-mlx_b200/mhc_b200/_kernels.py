@@ -17,7 +17,7 @@ from . import _capi as C
 
 F32 = torch.float32
 
-# Optional per-launch timing: when set to a dict, each timed C-ABI launch
+# Optional per-launch timing: when set to a dict, each C-ABI launch of this file
 # appends a (start, end) pair of CUDA events recorded on the launching
 # stream under the entry point's name.  Off (None) in normal use.
 TIMING: dict | None = None

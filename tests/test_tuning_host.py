@@ -173,3 +173,20 @@ def test_host_extension():
                 ([p], at(numel), 0, -1, at(out), at(out))):
         with pytest.raises(ValueError):
             host.gather(*bad)
+
+
+def test_host_calls_refuse_other_arguments():
+    host = _capi.host()
+    x, y = _rows()
+    for call in (host.linear, host.token_logprobs, host.logits_grad, host.preference, host.policy,
+                 host.bind):
+        with pytest.raises(TypeError):
+            call(x)
+    with pytest.raises(TypeError):
+        host.token_logprobs(x, 3, -100)
+    with pytest.raises(TypeError):
+        host.token_logprobs(x, y, "a")
+    with pytest.raises(RuntimeError, match="CUDA"):
+        host.token_logprobs(x, y, -100)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        host.linear(x, x, None, None, 0)
