@@ -343,7 +343,7 @@ MHC_API int mhc_qlinear_bwd_dx_t(const void* dy, int dy_dtype, const uint32_t* w
  * V contiguous values; targets[t] is its class, or ignore_index for a row that
  * takes no part.  A target outside [0, V) and a row without a finite logit
  * give NaN.  logp[t] = ln softmax(x_t)[targets[t]] (0 where ignored);
- * stats[t] = (max, 1 / sum exp(x - max), 1 - p of the target, scratch), four
+ * stats[t] = (max, 1 / sum exp(x - max), 1 - p of the target, logp's low part or scratch), four
  * floats a row (16-byte aligned), for mhc_logits_grad.  rows < 2^28.
  *   mhc_token_logprobs: logp and stats.
  *   mhc_logits_grad: dlogits[t, v] = c_t (1[v = targets[t]] - softmax(x_t)[v]),

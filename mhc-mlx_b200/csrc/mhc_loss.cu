@@ -357,8 +357,9 @@ template <typename T>
 __device__ __forceinline__ float target_logit(const T* x, int64_t y, int64_t V) {
   return (y >= 0 && y < V) ? to_f(x[y]) : CUDART_NAN_F;
 }
-// A row's record: m, 1 / S, R / S.  The fourth word is the i-th row to be worked on
-// (k_order), which has nothing to do with row i itself.
+// A row's record: m, 1 / S, R / S, and logp's low part.  Where rows are worked on in
+// order (k_order) the fourth word is instead the i-th row to be worked on, which
+// has nothing to do with row i itself, and is left alone.
 __device__ __forceinline__ void put_stats(float4* p, float m, float inv_s, float miss) {
   *reinterpret_cast<float2*>(p) = make_float2(m, inv_s);
   reinterpret_cast<float*>(p)[2] = miss;
@@ -367,14 +368,18 @@ __device__ __forceinline__ void put_stats(float4* p, float m, float inv_s, float
 // target's logit.  Without a finite logit, or with a NaN, +inf or a bad
 // target, all is NaN.
 struct RowEnd {
-  float logp, m, inv_s, miss;  // miss: 1 - p of the target
+  float logp, low, m, inv_s, miss;  // logp + low in more digits; miss: 1 - p of the target
 };
 __device__ __forceinline__ RowEnd row_end(float xt, MaxSum a) {
   const float m = fmaxf(xt, a.m);
   const float r = a.m == m ? a.s : a.s * exp_diff(a.m, m);
   const float e = xt == m ? 1.0f + (m - m) : exp_diff(xt, m);  // NaN where m is not finite
   const float s = r + e, inv = 1.0f / s, bad = s - s;
-  return {(xt == m ? -log1pf(r) : (xt - m) - logf(s)) + bad, m, inv, r * inv + bad};
+  // What is summed over a sequence or subtracted from another log probability
+  // should not lose logp's last digits to its rounding.
+  const double l = xt == m ? -log1p((double)r) : ((double)xt - (double)m) - log((double)s);
+  const float logp = (float)l + bad;
+  return {logp, isfinite(logp) ? (float)(l - (double)logp) : 0.f, m, inv, r * inv + bad};
 }
 
 __device__ __forceinline__ double block_sum_f64(double v, double* red) {
@@ -438,9 +443,9 @@ struct Policy {
 struct Token {
   float loss, kl, slope;
 };
-__device__ __forceinline__ Token policy_token(float logp, float old, float adv, float ref,
+__device__ __forceinline__ Token policy_token(float logp, float low, float old, float adv, float ref,
                                               const Policy& p) {
-  const float r = expf(logp - old);
+  const float r = expf((logp - old) + low);
   const float free = r * adv, held = fminf(fmaxf(r, p.clip_lo), p.clip_hi) * adv;
   Token k;
   // where the two agree (inside the clip) the gradient is the free one's
@@ -449,7 +454,7 @@ __device__ __forceinline__ Token policy_token(float logp, float old, float adv, 
   if (free != free) k.loss = k.slope = free;  // comparisons and fminf drop a NaN
   k.kl = 0.f;
   if (p.ref) {
-    const float d = ref - logp, em = expm1f(d);
+    const float d = (ref - logp) - low, em = expm1f(d);
     k.kl = em - d;
     if (p.kl_coef != 0.f) {
       k.loss += p.kl_coef * k.kl;
@@ -754,7 +759,7 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
       const RowEnd e = row_end(xt, acc);
       float c = 0.f;
       if constexpr (POLICY) {
-        const Token k = policy_token(e.logp, old, adv, ref, run.pol);
+        const Token k = policy_token(e.logp, e.low, old, adv, ref, run.pol);
         c = k.slope * *run.inv_d;
         if (tid == 0) {
           const float cg = c * run.grad_scale;
@@ -768,6 +773,7 @@ k_rows(const Rows a, int slice, int cs, int ordered, float* __restrict__ logp, f
       if (first) {
         logp[t] = e.logp;
         put_stats(stats + t, e.m, e.inv_s, e.miss);
+        if (!POLICY) stats[t].w = e.low;
         if (coef) coef[t] = c;
       }
     }
@@ -891,6 +897,7 @@ k_long_rows(Rows a, int slice, int cs, float* __restrict__ logp, float4* __restr
     const RowEnd e = row_end(xt, acc);
     logp[t] = e.logp;
     put_stats(stats + t, e.m, e.inv_s, e.miss);
+    stats[t].w = e.low;
   }
   cluster_arrive();
   cluster_wait();
@@ -907,6 +914,7 @@ struct Preference {
   int64_t uniform;
   int64_t pairs, rows;
   const float* logp;
+  const float4* stats;
   const float* ref;
   const int64_t* targets;
   int64_t ignore;
@@ -938,18 +946,19 @@ k_preference(Preference a, int cs, float* __restrict__ margins, float* __restric
     const int64_t lo = seq_offset(a, 2 * b + me), hi = seq_offset(a, 2 * b + me + 1);
     double v = 0.0;
     for (int64_t t = lo + tid; t < hi; t += kU * kSeqThreads) {
-      float d[kU], r[kU];
+      float d[kU], low[kU], r[kU];
       int64_t y[kU];
 #pragma unroll
       for (int u = 0; u < kU; ++u) {  // all asked for before the first is used
         const int64_t at = t + u * kSeqThreads < hi ? t + u * kSeqThreads : t;
         y[u] = a.targets[at];
         d[u] = a.logp[at];
+        low[u] = a.stats[at].w;
         r[u] = a.ref[at];
       }
 #pragma unroll
       for (int u = 0; u < kU; ++u)
-        if (t + u * kSeqThreads < hi && y[u] != a.ignore) v += (double)d[u] - (double)r[u];
+        if (t + u * kSeqThreads < hi && y[u] != a.ignore) v += ((double)d[u] - (double)r[u]) + (double)low[u];
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -1059,7 +1068,8 @@ k_logits_grad(Rows a, int64_t slice, int parts, const float4* __restrict__ stats
 // probabilities, by one block (k_long_rows before, k_logits_grad after).
 __global__ void __launch_bounds__(1024)
 k_policy_tokens(const int64_t* __restrict__ targets, int64_t ignore, int64_t rows, Policy pol,
-                const float* __restrict__ logp, const float* __restrict__ inv_d_ptr,
+                const float* __restrict__ logp, const float4* __restrict__ stats,
+                const float* __restrict__ inv_d_ptr,
                 float* __restrict__ coef, float* __restrict__ loss, float* __restrict__ kl) {
   __shared__ double red[32];
   const float inv_d = *inv_d_ptr;
@@ -1067,7 +1077,7 @@ k_policy_tokens(const int64_t* __restrict__ targets, int64_t ignore, int64_t row
   for (int64_t t = threadIdx.x; t < rows; t += 1024) {
     Token k = {0.f, 0.f, 0.f};
     if (targets[t] != ignore)
-      k = policy_token(logp[t], pol.old[t], pol.adv[t], pol.ref ? pol.ref[t] : 0.f, pol);
+      k = policy_token(logp[t], stats[t].w, pol.old[t], pol.adv[t], pol.ref ? pol.ref[t] : 0.f, pol);
     coef[t] = k.slope * inv_d;
     u += (double)k.loss;
     v += (double)k.kl;
@@ -1223,7 +1233,7 @@ int run_policy(const LogitsArg& l, const Policy& p, float inv_d, float scale, co
   k_order<<<1, 1024, 0, st>>>(l.targets, (int)l.rows, l.ignore, nullptr, inv_d, o.inv_d, o.ticket);
   r = check_launch("policy_loss");
   if (r != MHC_OK) return r;
-  k_policy_tokens<<<1, 1024, 0, st>>>(l.targets, l.ignore, l.rows, p, o.logp, o.inv_d, o.coef,
+  k_policy_tokens<<<1, 1024, 0, st>>>(l.targets, l.ignore, l.rows, p, o.logp, stats, o.inv_d, o.coef,
                                       o.loss, o.kl);
   r = check_launch("policy_loss");
   if (r != MHC_OK || !o.dlogits) return r;
@@ -1263,7 +1273,7 @@ static int run_preference(const LogitsArg& l, const PreferenceArg& a, const Pref
     const int r = run_stats<T>(l, o.logp, reinterpret_cast<float4*>(o.stats), o.coef, st);
     if (r != MHC_OK) return r;
   }
-  const Preference p = {a.cu_seqlens, a.cu_is64, a.uniform, a.pairs,  l.rows,      o.logp, a.ref,
+  const Preference p = {a.cu_seqlens, a.cu_is64, a.uniform, a.pairs,  l.rows,  o.logp, reinterpret_cast<const float4*>(o.stats), a.ref,
                         l.targets,    l.ignore,  a.beta,    a.smoothing, a.inv_d};
   int cs = 1;
   while (cs < kMaxCluster && cs < a.pairs) cs *= 2;
