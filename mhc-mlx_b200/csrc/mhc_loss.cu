@@ -577,7 +577,7 @@ k_order(const int64_t* __restrict__ targets, int rows, int64_t ignore, float4* _
 // about three times what 44 GB/s an SM needs in flight.
 //
 // Measured, 8192 rows of 32000 bf16 logits (524 MB), some of them ignored: loss
-// and gradient 176 us (160 us at the copy rate for the whole matrix in and
+// and gradient 181 us (160 us at the copy rate for the whole matrix in and
 // out; memory bound), the sums alone 88 us (80 us at the copy rate; the
 // exponential unit is 62 % busy and the rest of the issue slots' work waits
 // between rows).  A block a row that loads its row itself: loss and gradient 224 us.
