@@ -435,7 +435,7 @@ MHC_API int mhc_adamw_step(int count, void* const* params, const void* const* gr
  * row are contiguous, ld* is the distance between rows in elements.  act: 0 none,
  * 1 relu, 2 silu, 3 gelu (erf).  bias and residual may be NULL.
  * z (nullable in the forward; NULL in the backward for act 0) holds the
- * pre-activation rounded to the type, 16-byte aligned, ldz >= N a multiple of 8.
+ * pre-activation in fp32, 16-byte aligned, ldz >= N a multiple of 8.
  * dx, dw and dbias may each be NULL.  dz is rounded to the type before its
  * products.  Rows that do not begin on 16-byte boundaries are copied to padded
  * ones in the workspace.  1 <= N, K < 2^31; 0 <= M < 2^31 (M = 0 writes zeros
@@ -445,14 +445,14 @@ MHC_API size_t mhc_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const 
                                               int64_t ldw, int64_t M, int64_t N, int64_t K);
 MHC_API int mhc_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
                            const void* bias, const void* residual, int64_t ldr, int dtype,
-                           int act, void* z, int64_t ldz, void* y, int64_t ldy, int64_t M,
+                           int act, float* z, int64_t ldz, void* y, int64_t ldy, int64_t M,
                            int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
                            void* stream);
 MHC_API size_t mhc_linear_bwd_workspace_bytes(const void* dy, int64_t ldy, const void* x,
                                               int64_t ldx, const void* w, int64_t ldw, int act,
                                               int want_dx, int want_dw, int want_dbias,
                                               int64_t M, int64_t N, int64_t K);
-MHC_API int mhc_linear_bwd(const void* dy, int64_t ldy, const void* z, int64_t ldz,
+MHC_API int mhc_linear_bwd(const void* dy, int64_t ldy, const float* z, int64_t ldz,
                            const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
                            int act, void* dx, int64_t lddx, void* dw, int64_t lddw,
                            void* dbias, int64_t M, int64_t N, int64_t K, void* workspace,

@@ -666,7 +666,7 @@ size_t mhc_linear_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w,
 }
 
 int mhc_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
-                   const void* residual, int64_t ldr, int dtype, int act, void* z, int64_t ldz,
+                   const void* residual, int64_t ldr, int dtype, int act, float* z, int64_t ldz,
                    void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, void* workspace,
                    size_t workspace_bytes, void* stream) {
   MHC_TRY_BEGIN
@@ -704,7 +704,7 @@ size_t mhc_linear_bwd_workspace_bytes(const void* dy, int64_t ldy, const void* x
   return linear_bwd_ws_bytes(l);
 }
 
-int mhc_linear_bwd(const void* dy, int64_t ldy, const void* z, int64_t ldz, const void* x,
+int mhc_linear_bwd(const void* dy, int64_t ldy, const float* z, int64_t ldz, const void* x,
                    int64_t ldx, const void* w, int64_t ldw, int dtype, int act, void* dx,
                    int64_t lddx, void* dw, int64_t lddw, void* dbias, int64_t M, int64_t N,
                    int64_t K, void* workspace, size_t workspace_bytes, void* stream) {

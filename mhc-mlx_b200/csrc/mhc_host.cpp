@@ -131,7 +131,7 @@ struct Rows {
 };
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kHalf ? MHC_F16 : MHC_BF16; }
 
-// y, and with keep_z the pre-activation in rows padded to a multiple of 8.
+// y, and with keep_z the pre-activation in fp32, in rows padded to a multiple of 8.
 Tensor linear_fwd(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual,
                   int act, bool keep_z, Tensor* z) {
   const c10::cuda::CUDAGuard on(x.device());
@@ -142,11 +142,11 @@ Tensor linear_fwd(const Tensor& x, const Tensor& w, const Tensor& bias, const Te
   shape.back() = N;
   Tensor y = at::empty(shape, x.options());
   const int64_t ldz = (N + 7) / 8 * 8;
-  if (keep_z) *z = at::empty({M, ldz}, x.options());
+  if (keep_z) *z = at::empty({M, ldz}, x.options().dtype(at::kFloat));
   const size_t bytes = lib.fwd_bytes(ptr(xr.t), xr.ld, ptr(wr.t), wr.ld, M, N, K);
   const Tensor ws = workspace(bytes, x);
   check(lib.fwd(ptr(xr.t), xr.ld, ptr(wr.t), wr.ld, ptr(b), ptr(rr.t), rr.ld, dtype_of(x), act,
-                keep_z ? ptr(*z) : nullptr, ldz, ptr(y), N, M, N, K, ptr(ws), bytes, stream_of(x)),
+                keep_z ? z->data_ptr<float>() : nullptr, ldz, ptr(y), N, M, N, K, ptr(ws), bytes, stream_of(x)),
         "mhc_linear_fwd");
   return y;
 }
@@ -186,7 +186,8 @@ struct Linear : torch::autograd::Function<Linear> {
       const size_t bytes = lib.bwd_bytes(ptr(dr2.t), dr2.ld, ptr(xr.t), xr.ld, ptr(wr.t), wr.ld, act,
                                          want_dx, want_dw, want_db, M, N, K);
       const Tensor ws = workspace(bytes, x);
-      check(lib.bwd(ptr(dr2.t), dr2.ld, ptr(z), z.defined() ? z.size(1) : 0, ptr(xr.t), xr.ld,
+      check(lib.bwd(ptr(dr2.t), dr2.ld, z.defined() ? z.data_ptr<float>() : nullptr,
+                    z.defined() ? z.size(1) : 0, ptr(xr.t), xr.ld,
                     ptr(wr.t), wr.ld, dtype_of(x), act, ptr(dx), K, ptr(dw), K, ptr(db), M, N, K,
                     ptr(ws), bytes, stream_of(x)),
             "mhc_linear_bwd");

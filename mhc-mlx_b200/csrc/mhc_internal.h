@@ -255,7 +255,7 @@ struct LinearArg {
   int64_t ldx, ldw, ldr;
   int dtype, act;
   int64_t M, N, K;
-  void* z;  // nullable: the pre-activation, rows padded to a multiple of 8
+  void* z;  // nullable: the pre-activation in fp32, rows padded to a multiple of 8
   int64_t ldz;
   void* y;
   int64_t ldy;

@@ -8,7 +8,9 @@
 // reduction along their rows or down their columns (W in dx; both in dW), fp32
 // accumulators in tensor memory, bias, activation and residual applied as
 // they are read back: z never makes a round trip through memory, unless the
-// backward will want it (then it is written, rounded to the type, beside y).
+// backward will want it: then it is written in fp32 beside y.  In the operands'
+// type it would take half the room, but move a slope by up to 0.3 of the type's
+// rounding of dy, most where the slope goes through 0.
 //
 // k_gemm: one CTA an SM walks 128 x BN output tiles (BN 256, 128 or 64 by the
 // number of tiles):
@@ -83,7 +85,7 @@ template <typename T>
 struct Epilogue {
   const T* bias;      // [N], nullable
   const T* residual;  // [M][ldr], nullable
-  T* z;               // [M][ldz], nullable
+  float* z;           // [M][ldz], nullable
   T* d;               // [M][ldd]
   int64_t ldr, ldz, ldd;
   int M, N;
@@ -312,59 +314,71 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
       for (int c = c0; c < c1; c += 64) {
         const int col = n * BN + c, cols = min(64, ep.N - col);
         if (rows <= 0 || cols <= 0) break;
-        // y, then z where it is wanted: the accumulator is read for each
-#pragma unroll 1
-        for (int pass = 0; pass < (ep.z ? 2 : 1); ++pass) {
-          const bool res = pass == 0 && ep.residual != nullptr, staged = res && !ep.wide_res;
-          if (!staged || c != c0) {
-            if (lane == 0) tma_store_read();
-            __syncwarp();
+        // 32 of the 64 columns (half h), with the bias
+        const auto read_acc = [&](int h, float (&v)[32]) {
+          uint32_t r[32];
+          if (ok) tmem_ld32(tmem + ((uint32_t)(sp * 32) << 16) + (uint32_t)(buf * BN + c + 32 * h), r);
+          const float bl = c == c0 ? (h ? bias[1] : bias[0]) : (h ? bias[3] : bias[2]);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = ok ? __uint_as_float(r[e]) : CUDART_NAN_F;
+          if (ep.bias) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] += __shfl_sync(0xffffffffu, bl, e);
           }
-          if (staged && c != c0) {
-            rows_in(ep.residual + (int64_t)row0 * ep.ldr + col, ep.ldr, stage, lane, rows, cols);
-            __syncwarp();
-          }
+        };
+        const bool staged = ep.residual != nullptr && !ep.wide_res;
+        if (!staged || c != c0) {
+          if (lane == 0) tma_store_read();
+          __syncwarp();
+        }
+        if (staged && c != c0) {
+          rows_in(ep.residual + (int64_t)row0 * ep.ldr + col, ep.ldr, stage, lane, rows, cols);
+          __syncwarp();
+        }
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            uint32_t r[32];
-            if (ok) tmem_ld32(tmem + ((uint32_t)(sp * 32) << 16) + (uint32_t)(buf * BN + c + 32 * h), r);
-            const float bl = c == c0 ? (h ? bias[1] : bias[0]) : (h ? bias[3] : bias[2]);
+        for (int h = 0; h < 2; ++h) {
+          float a[32];
+          read_acc(h, a);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int e0 = 32 * h + 8 * q;
-              float v[8];
+          for (int q = 0; q < 4; ++q) {
+            const int e0 = 32 * h + 8 * q;
+            float v[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = ok ? __uint_as_float(r[8 * q + e]) : CUDART_NAN_F;
-              if (ep.bias) {
+            for (int e = 0; e < 8; ++e) v[e] = act_of<ACT>(a[8 * q + e]);
+            uint4* at = chunk_of(stage, lane, 4 * h + q);
+            if (ep.residual) {
+              float b[8];
+              if (staged) unpack16<T, 8>(*at, b);
+              else read8(ep.residual + (int64_t)(row0 + lane) * ep.ldr + col + e0, 1, lane < rows ? cols - e0 : 0, b);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += __shfl_sync(0xffffffffu, bl, 8 * q + e);
-              }
-              uint4* at = chunk_of(stage, lane, 4 * h + q);
-              if (pass == 0) {
-                if constexpr (ACT != kNone) {
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) v[e] = act_of<ACT>(v[e]);
-                }
-                if (res) {
-                  float b[8];
-                  if (staged) unpack16<T, 8>(*at, b);
-                  else read8(ep.residual + (int64_t)(row0 + lane) * ep.ldr + col + e0, 1, lane < rows ? cols - e0 : 0, b);
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) v[e] += b[e];
-                }
-              }
-              *at = pack8<T>(v);
+              for (int e = 0; e < 8; ++e) v[e] += b[e];
             }
+            *at = pack8<T>(v);
           }
-          if (pass == 1 || ep.wide_d) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) tma_store_2d(pass == 1 ? &map_z : &map_d, stage, col, row0);
-          } else {
-            __syncwarp();
-            rows_out(ep.d + (int64_t)row0 * ep.ldd + col, ep.ldd, stage, lane, rows, cols);
-            __syncwarp();
-          }
+        }
+        if (ep.wide_d) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tma_store_2d(&map_d, stage, col, row0);
+        } else {
+          __syncwarp();
+          rows_out(ep.d + (int64_t)row0 * ep.ldd + col, ep.ldd, stage, lane, rows, cols);
+          __syncwarp();
+        }
+        // z where it is wanted: the accumulator is read again, 32 columns fill the stage
+#pragma unroll 1
+        for (int h = 0; ep.z && 32 * h < cols && h < 2; ++h) {
+          float a[32];
+          read_acc(h, a);
+          if (lane == 0) tma_store_read();
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            *chunk_of(stage, lane, q) = make_uint4(__float_as_uint(a[4 * q]), __float_as_uint(a[4 * q + 1]),
+                                                   __float_as_uint(a[4 * q + 2]), __float_as_uint(a[4 * q + 3]));
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tma_store_2d(&map_z, stage, col + 32 * h, row0);
         }
       }
       tc_fence_before();
@@ -473,7 +487,7 @@ k_few_rows(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_
 #pragma unroll
     for (int p = 0; p < 8; ++p) v += part[p][f][tok];
     if (ep.bias) v += to_f(ep.bias[n]);
-    if (ep.z) ep.z[(int64_t)tok * ep.ldz + n] = from_f<T>(v);
+    if (ep.z) ep.z[(int64_t)tok * ep.ldz + n] = v;
     v = act_of<ACT>(v);
     if (ep.residual) v += to_f(ep.residual[(int64_t)tok * ep.ldr + n]);
     ep.d[(int64_t)tok * ep.ldd + n] = from_f<T>(v);
@@ -485,7 +499,7 @@ k_few_rows(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_
 // tile's column sums.  dz may be null (no activation, rows as TMA wants them).
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256)
-k_act_grad(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ z, int64_t ldz,
+k_act_grad(const T* __restrict__ dy, int64_t ldy, const float* __restrict__ z, int64_t ldz,
            T* __restrict__ dz, int64_t lddz, float* __restrict__ part, int64_t M, int N, int per, int wide_dy) {
   __shared__ float red[8][256];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -498,7 +512,7 @@ k_act_grad(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ z, int64
       read8(dy + m * ldy + col, wide_dy, left, d);
       if constexpr (ACT != kNone) {
         float v[8];
-        read8(z + m * ldz + col, true, ldz - col < 8 ? left : 8, v);  // z's rows are padded to 8
+        load_vec<float, 8>(z + m * ldz + col, v);  // z's rows are padded to 8
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[e] *= act_slope<ACT>(v[e]);
         if (left < 8) {
@@ -615,7 +629,7 @@ int run_gemm(const char* fn, const Matrix& a, const Matrix& b, const Epilogue<T>
   r = make_tensor_map(fn, &mb, dt, b.p, (uint64_t)b.cols, (uint64_t)b.rows, (uint64_t)b.ld * 2, 64,
                       BT ? 64 : BN, CU_TENSOR_MAP_SWIZZLE_128B);
   if (r != MHC_OK) return r;
-  // outputs: 64 columns x 32 rows a store; a map that is not used is the operand's
+  // outputs: 64 columns (z: 32) x 32 rows a store; a map that is not used is the operand's
   CUtensorMap md = ma, mz = ma;
   if (ep.wide_d) {
     r = make_tensor_map(fn, &md, dt, ep.d, (uint64_t)ep.N, (uint64_t)ep.M, (uint64_t)ep.ldd * 2, 64, 32,
@@ -623,8 +637,8 @@ int run_gemm(const char* fn, const Matrix& a, const Matrix& b, const Epilogue<T>
     if (r != MHC_OK) return r;
   }
   if (ep.z) {
-    r = make_tensor_map(fn, &mz, dt, ep.z, (uint64_t)ep.N, (uint64_t)ep.M, (uint64_t)ep.ldz * 2, 64, 32,
-                        CU_TENSOR_MAP_SWIZZLE_128B);
+    r = make_tensor_map(fn, &mz, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, ep.z, (uint64_t)ep.N, (uint64_t)ep.M,
+                        (uint64_t)ep.ldz * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
     if (r != MHC_OK) return r;
   }
   const auto kern = k_gemm<T, BN, AT, BT, ACT>;
@@ -692,7 +706,7 @@ int forward(const LinearArg& l, cudaStream_t st) {
   ep.bias = static_cast<const T*>(l.bias);
   ep.residual = static_cast<const T*>(l.residual);
   ep.ldr = l.ldr;
-  ep.z = static_cast<T*>(l.z);
+  ep.z = static_cast<float*>(l.z);
   ep.ldz = l.ldz;
   ep.wide_res = tma_rows(l.residual, l.ldr);
   if (l.M <= kFewRows) {
@@ -737,7 +751,7 @@ int backward(const LinearGradArg& l, cudaStream_t st) {
     }
     if (parts > 65535) return set_error(MHC_ERR_UNSUPPORTED, "%s: M=%lld is too large", fn, (long long)l.M);
     const dim3 grid((unsigned)((l.N + 255) / 256), (unsigned)parts);
-    k_act_grad<T, ACT><<<grid, 256, 0, st>>>(static_cast<const T*>(l.dy), l.ldy, static_cast<const T*>(l.z),
+    k_act_grad<T, ACT><<<grid, 256, 0, st>>>(static_cast<const T*>(l.dy), l.ldy, static_cast<const float*>(l.z),
                                              l.ldz, static_cast<T*>(q), up8(l.N), part, l.M, (int)l.N, per,
                                              tma_rows(l.dy, l.ldy));
     int r = check_launch(fn);

@@ -49,8 +49,9 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     x [..., in], weight [out, in], bias [out], residual [..., out], all bf16 or
     all fp16; activation "none", "relu", "silu" or "gelu".  Products and sums are
     fp32, rounded once to y.  The gradients are rounded once to their tensors'
-    type; with an activation the pre-activation (kept for the backward) and its
-    gradient (an operand of the products) are rounded to the type too."""
+    type; with an activation the pre-activation's gradient, an operand of the
+    products on the tensor cores, is rounded to the type too.  The pre-activation
+    is kept for the backward in fp32."""
     act = _check(x, weight, bias, residual, activation)
     return C.host().linear(x, weight, bias, residual, act)
 

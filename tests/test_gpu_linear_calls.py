@@ -1,0 +1,35 @@
+"""Calls of the linear layer that its kernels do not see, and its gradients' digits.
+Tolerances as in test_gpu_linear.py, but for the slope: it comes from the pre-activation in
+fp32, so nothing is allowed for a rounding of z."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+from test_gpu_linear import ACT, EPS, TINY, U, _make, _within
+
+from mhc_b200 import linear_act
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 64), (13, 1500, 72), (17, 1501, 72), (40, 2050, 100),
+                                   (300, 1000, 40), (1000, 777, 33)])
+def test_slopes_come_from_the_pre_activation_in_fp32(dtype, act, M, N, K):
+    """dbias is a sum of dz in fp32: u of itself, and the slope's own error.  A z rounded to
+    the type would add 0.3 u |dy| a row, most of it where the slope goes through 0."""
+    x, w, b, res, dy = _make(M, N, K, dtype, M + N)
+    bias = b.clone().requires_grad_(True)
+    y = linear_act(x, w, bias, residual=res, activation=act)
+    (db,) = torch.autograd.grad(y, bias, dy)
+    X, W, D = x.double(), w.double(), dy.double()
+    z = (X @ W.t() + b.double()).requires_grad_(True)
+    size = X.abs() @ W.abs().t() + b.double().abs()
+    (slope,) = torch.autograd.grad(ACT[act](z).sum(), z)
+    dz = D * slope
+    noise = EPS * D.abs() * (1 + size)
+    want = dz.sum(0)
+    _within(db, want, noise.sum(0) + EPS * dz.abs().sum(0) + U[dtype] * want.abs() + TINY[dtype] + 1e-30, "db")
