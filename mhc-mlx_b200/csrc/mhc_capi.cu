@@ -580,10 +580,10 @@ int mhc_preference_loss(const void* logits, int dtype, int64_t rows, int64_t row
 }
 
 // Workspace of the policy loss: a counter and 1 / D, then two fp64 sums for
-// each cluster of blocks (at most 8 blocks of 128 threads an SM).
+// each cluster of blocks.
 static constexpr size_t kLossHeader = 256;
 size_t mhc_policy_workspace_bytes(void) {
-  return kLossHeader + (size_t)sm_count() * 8 * 2 * sizeof(double);
+  return kLossHeader + (size_t)sm_count() * kPolicyClustersSM * 2 * sizeof(double);
 }
 
 int mhc_policy_loss(const void* logits, int dtype, int64_t rows, int64_t rows_per_batch,

@@ -217,6 +217,8 @@ struct PolicyArg {
   const float *old, *adv, *ref;  // ref null: no KL term
   float clip_low, clip_high, kl_coef, inv_d, grad_scale;  // inv_d 0: 1 / valid tokens
 };
+// Clusters of blocks to an SM, at most, whose sums the policy loss's workspace holds.
+constexpr int kPolicyClustersSM = 8;
 struct PolicyOut {
   float *logp, *stats, *coef, *loss, *kl;
   // workspace: a counter, 1 / D, and two sums a cluster of blocks

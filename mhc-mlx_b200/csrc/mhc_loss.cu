@@ -609,7 +609,7 @@ struct PolicyRun {
 template <bool POLICY>
 struct RowShape {
   static constexpr int kNV = POLICY ? 8 : 16;
-  static constexpr int kThreadsSM = POLICY ? 1024 : 768;
+  static constexpr int kThreadsSM = POLICY ? 128 * kPolicyClustersSM : 768;
 };
 template <typename T, int NT, bool POLICY>
 __global__ void __launch_bounds__(NT, RowShape<POLICY>::kThreadsSM / NT)
@@ -1167,6 +1167,9 @@ int run_rows_nt(const char* what, const LogitsArg& l, const Split& sp, float* lo
   int64_t clusters = (int64_t)sm_count() * blocks_per_sm(kern, NT, smem) / sp.cs;
   if (clusters < 1) clusters = 1;
   if (clusters > l.rows) clusters = l.rows;
+  // each has its pair of sums in the workspace, whatever number of blocks fits
+  if (POLICY && clusters > (int64_t)sm_count() * kPolicyClustersSM)
+    clusters = (int64_t)sm_count() * kPolicyClustersSM;
   // the order pays where the rows' work is what counts: 8192 rows of 32000 bf16,
   // 30 % ignored, 187 us by number and 172 in order; reading alone gains 7 us of
   // 98 and would pay a launch for it
