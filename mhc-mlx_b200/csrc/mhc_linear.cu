@@ -239,8 +239,9 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
           }
         }
       }
-      if (*abort_flag)  // copies in flight land before the CTA's shared memory goes away
-        for (int i = it - S < 0 ? 0 : it - S; i < it; ++i) (void)mbar_wait(&full[i % S], (unsigned)(i / S) & 1u);
+      // copies in flight land before the CTA's shared memory goes away: the MMAs have
+      // waited for them, unless some wait has run out (this loop may have ended before)
+      for (int i = it - S < 0 ? 0 : it - S; i < it; ++i) (void)mbar_wait(&full[i % S], (unsigned)(i / S) & 1u);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA --
@@ -270,6 +271,8 @@ k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtens
         umma_commit(&acc_full[buf]);  // also after an abort: marks the issued MMAs' completion
         if (!ok) {
           s_abort = 1;
+          // they still read shared memory and write the accumulators that are freed below
+          (void)mbar_wait(&acc_full[buf], (unsigned)(i >> 1) & 1u);
           break;
         }
       }
