@@ -40,6 +40,12 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _apart(params) -> bool:
+    """Whether no two of them share memory: blocks of one launch would race for it."""
+    spans = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in params if p.numel())
+    return all(a + size <= b for (a, size), (b, _) in zip(spans, spans[1:]))
+
+
 class _States(dict):
     """Optimizer.state: a parameter's views of the flat buffers are made when they are
     first asked for (hundreds of parameters, four buffers each)."""
@@ -175,7 +181,8 @@ class AdamW(torch.optim.Optimizer):
         p = (1 - lr weight_decay) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
     params: as for torch.optim.AdamW (groups may set lr, betas, eps and
-      weight_decay).  Each is dense in memory, in any order of its axes.
+      weight_decay).  Each is dense in memory, in any order of its axes, and none
+      shares memory with another of its group.
     state_bits: 32, or 8 for moments of a byte an element.
     master_weights: keep 16-bit parameters in fp32 beside them; updates are made
       on those and the parameter receives the rounded values.
@@ -218,6 +225,8 @@ class AdamW(torch.optim.Optimizer):
             by.setdefault((p.dtype, p.device), []).append(p)
         packs = []
         for k, ((dtype, _), ps) in enumerate(by.items()):
+            if not _apart(ps):
+                raise ValueError("parameters of a group share memory")
             pack = _Pack(ps, self.state_bits, self.master_weights and dtype != torch.float32,
                          64 * index + k)
             packs.append(pack)
