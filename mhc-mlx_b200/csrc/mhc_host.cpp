@@ -4,6 +4,7 @@
 //   gather   what an optimizer step asks of hundreds of tensors: 512 parameters'
 //            and gradients' sizes, types, devices, layouts and addresses take
 //            some 250 us one attribute at a time, 10 us here.
+//   changed  the versions of what that step has written.
 //   linear   the linear layer over the C ABI, and its place in autograd: the
 //            engine calls a backward that is written in Python with the
 //            interpreter's lock, on a thread of its own.
@@ -462,6 +463,23 @@ PyObject* gather(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   Py_RETURN_TRUE;
 }
 
+// changed(tensors): a list of tensors whose values a kernel has written through their
+// addresses.  Their versions go up, as a torch operation in place would raise them: a
+// graph that saved one of them can tell.
+PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  const Args in("changed", args, nargs, 1);
+  TORCH_CHECK_TYPE(PyList_CheckExact(args[0]), "changed: a list is expected");
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(args[0]); ++i) {
+    PyObject* o = PyList_GET_ITEM(args[0], i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), "changed: a list of tensors is expected");
+    const Tensor& t = THPVariable_Unpack(o);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // those have no version
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
 }
@@ -474,6 +492,7 @@ PyMethodDef methods[] = {
     {"linear", fast(linear), METH_FASTCALL, "linear(x, weight, bias, residual, act) -> Tensor"},
     {"gather", fast(gather), METH_FASTCALL,
      "gather(params, numel, dtype, device, p_out, g_out) -> bool"},
+    {"changed", fast(changed), METH_FASTCALL, "changed(tensors): raises their versions"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mhc_host", nullptr, -1, methods};
 

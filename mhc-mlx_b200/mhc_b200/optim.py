@@ -122,6 +122,7 @@ class _Pack:
             if self.total:
                 self._call(group, t, seed, grad_scale, n, self.p_ptr, self.g_ptr, self.numel,
                            self.off)
+                C.host().changed([*self.params, *self.buffers.values()])
             return
         # parameters without a gradient, gradients in another order, or an error
         self._check_forms()
@@ -142,6 +143,7 @@ class _Pack:
                        (ctypes.c_int64 * k)(*(self.offsets[i] for i in which)))
             for i in which:
                 self.steps[i] = t + 1
+            C.host().changed([*(self.params[i] for i in which), *self.buffers.values()])
 
     def _check_forms(self) -> None:
         """The kernel goes by the sizes, type, device and layout that the state was made
