@@ -251,7 +251,16 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: torch.Tensor | None = None):
         """One update.  grad_scale: a device scalar that the gradients are multiplied by
-        (an inverse loss scale, a clipping coefficient), read by the kernel."""
+        (an inverse loss scale, a clipping coefficient), read by the kernel.
+
+        A step cannot be captured in a CUDA graph: replays would repeat its bias
+        corrections and its rounding."""
+        for packs in self._packs:
+            for pack in packs:
+                with K._on(pack.device):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("an AdamW step cannot be captured: its count of steps is "
+                                           "an argument of the kernel, the same at every replay")
         loss = None
         if closure is not None:
             with torch.enable_grad():

@@ -6,7 +6,7 @@ from __future__ import annotations
 
 import pytest
 import torch
-from test_gpu_adamw import HYPER
+from test_gpu_adamw import HYPER, _params, _set_grads
 
 import mhc_b200
 
@@ -44,6 +44,23 @@ def test_a_step_between_two_backwards_of_a_linear_layer():
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_capture_is_refused():
+    """A captured step would repeat one step's bias corrections and rounding."""
+    (p,) = _params([(300,)], torch.float32, 1)
+    opt = mhc_b200.AdamW([p], state_bits=8, **HYPER)
+    _set_grads([p], 2)
+    opt.step()
+    before = p.detach().clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(g):
+            opt.step()
+    assert opt.state_dict()["state"][0]["step"] == 1 and torch.equal(p.detach(), before)
+    opt.step()
+    assert not torch.equal(p.detach(), before)
 
 
 def test_parameters_that_share_memory_are_refused():
