@@ -122,7 +122,8 @@ class _Pack:
             if self.total:
                 self._call(group, t, seed, grad_scale, n, self.p_ptr, self.g_ptr, self.numel,
                            self.off)
-                C.host().changed([*self.params, *self.buffers.values()])
+                C.host().changed(self.params)
+                C.host().changed(list(self.buffers.values()))
             return
         # parameters without a gradient, gradients in another order, or an error
         self._check_forms()
