@@ -3,10 +3,11 @@ types' ranges.  Tolerances as in test_gpu_adamw.py."""
 
 from __future__ import annotations
 
+import math
 
 import pytest
 import torch
-from test_gpu_adamw import HYPER, _params, _set_grads
+from test_gpu_adamw import HYPER, _check_p, _hash, _params, _quantise, _set_grads
 
 import mhc_b200
 
@@ -61,6 +62,40 @@ def test_capture_is_refused():
     assert opt.state_dict()["state"][0]["step"] == 1 and torch.equal(p.detach(), before)
     opt.step()
     assert not torch.equal(p.detach(), before)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+@pytest.mark.parametrize("size", [1e-21, 1e-20, 1e-19, 1e-18, 1e-15])
+def test_8_bit_state_of_small_gradients(eps, size):
+    """v down among fp32's subnormal numbers: codes as the formulas give them, and a
+    parameter that moves by what m and the root of v come to."""
+    h = dict(HYPER, eps=eps)
+    (p,) = _params([(600,)], torch.float32, 3)
+    opt = mhc_b200.AdamW([p], state_bits=8, seed=7, **h)
+    buf = opt.state_buffers()
+    b1, b2 = h["betas"]
+    f32 = lambda v: torch.tensor(v, dtype=torch.float32, device=DEV)  # noqa: E731
+    for t in range(1, 4):
+        sign = torch.where(torch.arange(600, device=DEV) % 3 == 0, -1.0, 1.0)
+        p.grad = size * sign * (1 + torch.arange(600, device=DEV) % 7 / 8)
+        wide = lambda k: buf[k].float().view(-1, 256) * buf[k + "_scale"][:, None]  # noqa: E731
+        g = torch.zeros(768, device=DEV)
+        g[:600] = p.grad
+        g = g.view(-1, 256)
+        m = wide("exp_avg") * f32(b1) + g * f32(1 - b1)
+        r = wide("exp_avg_sq_root")
+        r = (r * r * f32(b2) + g * g * f32(1 - b2)).sqrt()
+        base = p.detach().double()
+        opt.step()
+        k = _hash(torch.arange(768, device=DEV), (7 * 0x9E3779B9 + t * 0x85A308D3) & 0xFFFFFFFF)
+        for key, x, u, floor in (("exp_avg", m, k & 0xFFFF, False),
+                                 ("exp_avg_sq_root", r, k >> 16, True)):
+            q, scale = _quantise(x, u, floor)
+            assert torch.equal(buf[key + "_scale"], scale), key
+            assert torch.equal(buf[key].float().view(-1, 256), q), key
+        mm, rr = (x.view(-1)[:600].double() for x in (m, r))
+        u = h["lr"] / (1 - b1 ** t) * mm / (rr / math.sqrt(1 - b2 ** t) + eps)
+        _check_p(p, base * (1 - h["lr"] * h["weight_decay"]) - u, u)
 
 
 def test_parameters_that_share_memory_are_refused():
