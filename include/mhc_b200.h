@@ -412,8 +412,10 @@ MHC_API int mhc_policy_loss(const void* logits, int dtype, int64_t rows, int64_t
  * state_bits 32: exp_avg (m) and exp_avg_sq (v) are fp32, the scales NULL.
  * state_bits 8: they hold e4m3 codes of m and of sqrt(v) in units of
  * exp_avg_scale[e / 256] / exp_avg_sq_scale[e / 256], powers of two; rounding is
- * up or down by a hash of the element's place in the state and `key`.  The
- * moments of a non-finite gradient become NaN and stay so.
+ * up or down by a hash of the element's place in the state and `key`.  A NaN
+ * code of sqrt(v) stands for infinity: a gradient above 1.8e19, whose square
+ * overflows, leaves its element where it is from then on but for the decay, as
+ * with 32 bits.  m of a non-finite gradient becomes NaN and stays so.
  * master (nullable, 16-bit parameters): fp32 weights that the update is made
  * on; the parameter receives their rounded values.
  * State buffers and master are 16-byte aligned. */

@@ -192,7 +192,8 @@ class AdamW(torch.optim.Optimizer):
     seed: of the 8-bit state's rounding.
 
     A parameter without a gradient is left alone.  A non-finite gradient makes its
-    element NaN for good: skip such steps (torch.amp.GradScaler does)."""
+    element NaN for good: skip such steps (torch.amp.GradScaler does).  One whose
+    square overflows (above 1.8e19) makes v infinite: its element then only decays."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, master_weights: bool = False,

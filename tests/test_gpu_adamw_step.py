@@ -98,6 +98,33 @@ def test_8_bit_state_of_small_gradients(eps, size):
         _check_p(p, base * (1 - h["lr"] * h["weight_decay"]) - u, u)
 
 
+@pytest.mark.parametrize("size", [2e19, 3e38])
+def test_a_gradient_whose_square_overflows(size):
+    """v is infinite: the element stays where it is but for the decay, with 8-bit state as
+    with 32."""
+    ps = [torch.nn.Parameter(torch.ones(512, device=DEV)) for _ in range(2)]
+    opts = [mhc_b200.AdamW([p], state_bits=b, lr=0.5, weight_decay=0.25) for p, b in zip(ps, (32, 8))]
+    rest = torch.arange(512, device=DEV) != 300
+    for t in range(20):
+        for p, opt in zip(ps, opts):
+            p.grad = torch.ones_like(p)
+            if t == 0:
+                p.grad[300] = size
+            opt.step()
+            assert torch.isfinite(p).all()
+            if t == 0:  # a decay of 1/8 and, elsewhere, a first step of lr
+                assert float(p.detach()[300]) == 0.875
+                assert ((p.detach()[rest] - 0.375).abs() <= 2.0 ** -20).all()
+        assert torch.equal(ps[0].detach()[300], ps[1].detach()[300])
+    # a gradient that is itself infinite is NaN for good
+    (p,) = ps[1:]
+    p.grad[300] = float("inf")
+    for _ in range(3):
+        opts[1].step()
+        p.grad = torch.ones_like(p)
+        assert torch.isnan(p[300]) and torch.isfinite(p[:256]).all()
+
+
 def test_parameters_that_share_memory_are_refused():
     """Blocks of one launch would write the same values."""
     p = torch.nn.Parameter(torch.zeros(10, device=DEV))
