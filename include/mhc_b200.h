@@ -417,7 +417,9 @@ MHC_API int mhc_policy_loss(const void* logits, int dtype, int64_t rows, int64_t
  * overflows, leaves its element where it is from then on but for the decay, as
  * with 32 bits.  m of a non-finite gradient becomes NaN and stays so.
  * master (nullable, 16-bit parameters): fp32 weights that the update is made
- * on; the parameter receives their rounded values.
+ * on; the parameter receives their rounded values.  Where the parameter is not
+ * its master's rounding when the call is made, it has been given another value,
+ * and the update starts from that.
  * State buffers and master are 16-byte aligned. */
 MHC_API int mhc_adamw_step(int count, void* const* params, const void* const* grads,
                            const int64_t* numel, const int64_t* offsets, int dtype,

@@ -188,7 +188,8 @@ class AdamW(torch.optim.Optimizer):
       shares memory with another of its group.
     state_bits: 32, or 8 for moments of a byte an element.
     master_weights: keep 16-bit parameters in fp32 beside them; updates are made
-      on those and the parameter receives the rounded values.
+      on those and the parameter receives the rounded values.  A parameter that has
+      been given other values since (a checkpoint) goes on from them.
     seed: of the 8-bit state's rounding.
 
     A parameter without a gradient is left alone.  A non-finite gradient makes its

@@ -7,7 +7,7 @@ import math
 
 import pytest
 import torch
-from test_gpu_adamw import HYPER, _check_p, _hash, _params, _quantise, _set_grads
+from test_gpu_adamw import HYPER, _check_p, _gen, _hash, _params, _quantise, _ref_step, _set_grads
 
 import mhc_b200
 
@@ -123,6 +123,46 @@ def test_a_gradient_whose_square_overflows(size):
         opts[1].step()
         p.grad = torch.ones_like(p)
         assert torch.isnan(p[300]) and torch.isfinite(p[:256]).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_new_values_of_a_parameter_with_a_master(bits, dtype):
+    """Values written into the parameter between steps are what the next step starts from;
+    elements that were left alone, or given the value that they had, keep their master's
+    digits."""
+    shapes = [(33, 50), (7,)]
+    params = _params(shapes, dtype, 1)
+    opt = mhc_b200.AdamW(params, state_bits=bits, master_weights=True, **HYPER)
+    _set_grads(params, 2)
+    opt.step()
+    fresh = torch.randn(33, 50, device=DEV, generator=_gen(4)).to(dtype)
+    fresh[0, :10] = params[0].detach()[0, :10]
+    with torch.no_grad():
+        params[0][:20].copy_(fresh[:20])
+        params[1].data = torch.full_like(params[1], 3.0)
+    start = [opt.state[p]["master"].double() for p in params]
+    kept = params[0].detach()[20:].clone()
+    assert torch.equal(start[0][20:].to(dtype), kept) and not torch.equal(start[0][20:], kept.double())
+    given = start[0][:20].to(dtype) != fresh[:20]
+    assert not given[0, :10].any() and given.sum() > 900
+    start[0][:20][given], start[1][:] = fresh[:20][given].double(), 3.0
+    own = [opt.state[p] for p in params]
+    if bits == 32:
+        m = [s["exp_avg"].double() for s in own]
+        v = [s["exp_avg_sq"].double() for s in own]
+    else:
+        b = opt.state_buffers()
+        wide = lambda k: (b[k].float().view(-1, 256) * b[k + "_scale"][:, None]).view(-1)  # noqa: E731
+        cut = lambda x: [x[:1650].view(33, 50).double(), x[1792:1799].double()]  # noqa: E731
+        m, v = cut(wide("exp_avg")), [r.square() for r in cut(wide("exp_avg_sq_root"))]
+    _set_grads(params, 3)
+    opt.step()
+    for p, x, mm, vv, s in zip(params, start, m, v, own):
+        want, _, _, u = _ref_step(x, p.grad.double(), mm, vv, 2, HYPER)
+        _check_p(p, want, u)
+        tol = 2.0 ** -22 * want.abs() + 2.0 ** -19 * u.abs()
+        assert ((s["master"].double() - want).abs() <= tol).all()
 
 
 def test_parameters_that_share_memory_are_refused():
