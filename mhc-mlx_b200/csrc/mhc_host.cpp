@@ -60,7 +60,13 @@ Tensor workspace(size_t bytes, const Tensor& like) {
   return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
 }
 
-// All on x's device, which is a GPU; undefined ones do not count.
+// Outputs carry no tangent of forward-mode differentiation: one that came in would be
+// taken for 0.
+void require_no_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(),
+                              "mhc_b200: no forward-mode differentiation of this operator");
+}
+// All on x's device, which is a GPU, and without a tangent; undefined ones do not count.
 void require_cuda(const Tensor& x, std::initializer_list<const Tensor*> others) {
   TORCH_CHECK(lib.fwd != nullptr, "the library is not loaded");
   const auto one = [&](const Tensor& t) {
@@ -69,6 +75,7 @@ void require_cuda(const Tensor& x, std::initializer_list<const Tensor*> others) 
                 t.device(), ".  There is no CPU fallback.");
     TORCH_CHECK_VALUE(t.device() == x.device(), "tensors on different devices: ", x.device(), " and ",
                       t.device());
+    require_no_tangent(t);
   };
   one(x);
   for (const Tensor* t : others) one(*t);
@@ -175,6 +182,7 @@ struct Linear : torch::autograd::Function<Linear> {
     const bool want_dx = ctx->needs_input_grad(0), want_dw = ctx->needs_input_grad(1);
     const bool want_db = has_bias && ctx->needs_input_grad(2);
     Tensor dx, dw, db, dr;
+    if (dy.defined()) require_no_tangent(dy);
     if (want_dx || want_dw || want_db) {
       const bool twice = at::GradMode::is_enabled();
       const at::AutoGradMode off(false);

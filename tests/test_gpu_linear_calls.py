@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from test_gpu_linear import ACT, EPS, TINY, U, _make, _within
 
 from mhc_b200 import linear_act
@@ -33,3 +34,22 @@ def test_slopes_come_from_the_pre_activation_in_fp32(dtype, act, M, N, K):
     noise = EPS * D.abs() * (1 + size)
     want = dz.sum(0)
     _within(db, want, noise.sum(0) + EPS * dz.abs().sum(0) + U[dtype] * want.abs() + TINY[dtype] + 1e-30, "db")
+
+
+def test_forward_mode_is_refused():
+    """An output without a tangent would be taken for a constant."""
+    x, w, b, res, dy = _make(20, 24, 16, torch.bfloat16, 1)
+    for i in range(4):
+        for M in (1, 20):
+            for grad in (False, True):
+                with fwAD.dual_level(), torch.set_grad_enabled(grad):
+                    ts = [x[:M], w, b, res[:M]]
+                    ts[i] = fwAD.make_dual(ts[i], torch.ones_like(ts[i]))
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        linear_act(*ts[:3], residual=ts[3], activation="silu")
+    with fwAD.dual_level():
+        linear_act(x, w, b, residual=res)  # none of them dual
+        leaf = x.clone().requires_grad_()
+        y = linear_act(leaf, w)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, leaf, fwAD.make_dual(dy, torch.ones_like(dy)))

@@ -5,9 +5,11 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 from test_gpu_losses import (IGN, _check_grad, _logits, _logp_tol, _policy_inputs, _policy_ref,
                              _policy_tol, _ref_logp)
 
+import mhc_b200
 from mhc_b200 import _capi
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +32,18 @@ def test_policy_workspace_is_large_enough(dtype, V):
                None, 0.2, 0.2, 0.0, 0.0, 1.0, p(logp), p(stats), p(coef), p(loss), p(kl), None, p(ws),
                size, torch.cuda.current_stream().cuda_stream)
     assert (ws[size:] == 0xA5).all() and torch.isfinite(loss)
+
+
+def test_forward_mode_is_refused():
+    x, y = _logits((6, 40), F32, 1)
+    z = torch.zeros(6, device=DEV)
+    cu = torch.tensor([0, 3, 6], device=DEV)
+    with fwAD.dual_level():
+        d, e = (fwAD.make_dual(t, torch.ones_like(t)) for t in (x, z))
+        for call in (lambda: mhc_b200.token_logprobs(d, y), lambda: mhc_b200.preference_loss(d, y, z, cu),
+                     lambda: mhc_b200.preference_loss_grad(d, y, z, cu),
+                     lambda: mhc_b200.preference_loss_grad(x, y, e, cu),
+                     lambda: mhc_b200.policy_loss(d, y, z, z), lambda: mhc_b200.policy_loss_grad(d, y, z, z),
+                     lambda: mhc_b200.policy_loss_grad(x, y, z, e)):
+            with pytest.raises(RuntimeError, match="forward-mode|jvp"):
+                call()
