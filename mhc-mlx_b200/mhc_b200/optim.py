@@ -40,6 +40,11 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _alike(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one shape have their elements in one order in memory."""
+    return all(s == t for n, s, t in zip(a.shape, a.stride(), b.stride()) if n > 1) or not a.numel()
+
+
 def _apart(params) -> bool:
     """Whether no two of them share memory: blocks of one launch would race for it."""
     spans = sorted((p.data_ptr(), p.numel() * p.element_size()) for p in params if p.numel())
@@ -330,6 +335,9 @@ class AdamW(torch.optim.Optimizer):
             own = where[p][0].state_of(where[p][1])
             if set(saved) != {"step", *own} or any(saved[n].shape != v.shape for n, v in own.items()):
                 raise ValueError("loaded state does not fit its parameter")
+            # scales belong to blocks of memory
+            if self.state_bits == 8 and not all(_alike(saved[n], v) for n, v in own.items()):
+                raise ValueError("loaded 8-bit state is laid out otherwise than its parameter")
         for p, saved in pairs:
             pack, i = where[p]
             for n, v in pack.state_of(i).items():

@@ -177,3 +177,26 @@ def test_parameters_that_share_memory_are_refused():
     with pytest.raises(ValueError, match="share memory"):
         mhc_b200.AdamW([part(0, 100), part(10, 20), torch.nn.Parameter(flat[30:30])])
     mhc_b200.AdamW([part(50, 100), part(10, 50), part(0, 10), torch.nn.Parameter(flat[30:30])])
+
+
+def test_8_bit_state_of_another_layout_is_refused():
+    """Its scales go by blocks of memory, which hold other elements there."""
+    w = torch.randn(40, 30, device=DEV)
+    a, b = torch.nn.Parameter(w.t()), torch.nn.Parameter(w.t().contiguous())
+    for bits in (8, 32):
+        oa, ob = (mhc_b200.AdamW([x], state_bits=bits) for x in (a, b))
+        a.grad = torch.randn(30, 40, device=DEV)
+        oa.step()
+        saved = oa.state_dict()
+        if bits == 8:
+            with pytest.raises(ValueError, match="laid out"):
+                ob.load_state_dict(saved)
+            assert ob.state_dict()["state"][0]["step"] == 0
+        else:
+            ob.load_state_dict(saved)
+            assert torch.equal(ob.state[b]["exp_avg"], oa.state[a]["exp_avg"])
+    # an axis of one element has any stride
+    c = torch.nn.Parameter(torch.zeros(1, 8, device=DEV).t())
+    d = torch.nn.Parameter(torch.zeros(8, 1, device=DEV))
+    oc, od = (mhc_b200.AdamW([x], state_bits=8) for x in (c, d))
+    od.load_state_dict(oc.state_dict())
