@@ -109,6 +109,9 @@ class QuantizedLinear(nn.Module):
 
     @classmethod
     def from_linear(cls, linear: nn.Linear, group_size: int = 64, bits: int = 4):
+        if getattr(linear, "activation", "none") != "none":  # FusedLinear's
+            raise ValueError(f"QuantizedLinear has no activation, got a layer with "
+                             f"{linear.activation!r}")
         out_d, in_d = linear.weight.shape
         dtype = linear.weight.dtype if linear.weight.dtype != torch.float32 else torch.float16
         ql = cls(in_d, out_d, bias=linear.bias is not None, group_size=group_size, bits=bits,

@@ -5,7 +5,15 @@ from __future__ import annotations
 import pytest
 import torch
 
-from mhc_b200 import _capi
+from mhc_b200 import FusedLinear, QuantizedLinear, _capi
+
+
+def test_a_quantized_layer_keeps_no_activation():
+    """QuantizedLinear has no activation: a FusedLinear with one is refused, not stripped of it."""
+    plain = FusedLinear(64, 64, dtype=torch.float32)
+    QuantizedLinear.from_linear(plain)
+    with pytest.raises(ValueError, match="activation"):
+        QuantizedLinear.from_linear(FusedLinear(64, 64, activation="silu", dtype=torch.float32))
 
 
 def test_versions_go_up():
