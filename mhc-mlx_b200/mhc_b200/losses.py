@@ -75,8 +75,10 @@ def _check_per_token(name, t, targets):
 
 
 def _inverse(denominator) -> float:
-    if not denominator > 0:
-        raise ValueError(f"denominator must be positive, got {denominator}")
+    # its inverse is an fp32 argument of the kernels, where 0 means the number of tokens
+    if not 2.0 ** -126 <= denominator <= 2.0 ** 126:
+        raise ValueError(f"denominator must be positive, and its inverse an fp32 number, got "
+                         f"{denominator}")
     return 1.0 / float(denominator)
 
 

@@ -5,7 +5,21 @@ from __future__ import annotations
 import pytest
 import torch
 
+import mhc_b200
 from mhc_b200 import FusedLinear, QuantizedLinear, _capi
+
+
+@pytest.mark.parametrize("bad", [float("inf"), 1e39, 1e300, 1e-39, float("nan")])
+def test_denominators_whose_inverse_is_no_fp32_number(bad):
+    """The inverse goes to the kernels in fp32, where 0 stands for the number of tokens."""
+    x, y, z = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64), torch.zeros(4)
+    cu = torch.tensor([0, 2, 4])
+    for f in (mhc_b200.policy_loss, mhc_b200.policy_loss_grad):
+        with pytest.raises(ValueError, match="denominator"):
+            f(x, y, z, z, denominator=bad)
+    for f in (mhc_b200.preference_loss, mhc_b200.preference_loss_grad):
+        with pytest.raises(ValueError, match="denominator"):
+            f(x, y, z, cu, denominator=bad)
 
 
 def test_a_quantized_layer_keeps_no_activation():
