@@ -123,12 +123,12 @@ class _Pack:
                                           at(self.p_ptr), at(self.g_ptr)) \
                 and self.steps.count(self.steps[0]) == n:
             t = self.steps[0] + 1
-            self.steps = [t] * n
             if self.total:
                 self._call(group, t, seed, grad_scale, n, self.p_ptr, self.g_ptr, self.numel,
                            self.off)
                 C.host().changed(self.params)
                 C.host().changed(list(self.buffers.values()))
+            self.steps = [t] * n
             return
         # parameters without a gradient, gradients in another order, or an error
         self._check_forms()

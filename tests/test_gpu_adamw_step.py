@@ -165,6 +165,15 @@ def test_new_values_of_a_parameter_with_a_master(bits, dtype):
         assert ((s["master"].double() - want).abs() <= tol).all()
 
 
+def test_a_step_that_raises_does_not_count():
+    (p,) = _params([(30,)], torch.float32, 1)
+    opt = mhc_b200.AdamW([p], **HYPER)
+    _set_grads([p], 2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        opt.step(grad_scale=torch.ones(1))
+    assert opt.state_dict()["state"][0]["step"] == 0
+
+
 def test_parameters_that_share_memory_are_refused():
     """Blocks of one launch would write the same values."""
     p = torch.nn.Parameter(torch.zeros(10, device=DEV))
