@@ -263,6 +263,11 @@ class AdamW(torch.optim.Optimizer):
 
         A step cannot be captured in a CUDA graph: replays would repeat its bias
         corrections and its rounding."""
+        if grad_scale is not None and not (isinstance(grad_scale, torch.Tensor)
+                                           and grad_scale.numel() == 1):
+            raise ValueError("grad_scale must be a CUDA tensor of one number, got "
+                             + (f"shape {tuple(grad_scale.shape)}"
+                                if isinstance(grad_scale, torch.Tensor) else repr(grad_scale)))
         for packs in self._packs:
             for pack in packs:
                 with K._on(pack.device):

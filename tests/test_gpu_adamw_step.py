@@ -165,6 +165,19 @@ def test_new_values_of_a_parameter_with_a_master(bits, dtype):
         assert ((s["master"].double() - want).abs() <= tol).all()
 
 
+def test_grad_scale_is_one_number():
+    (p,) = _params([(30,)], torch.float32, 1)
+    opt = mhc_b200.AdamW([p], **HYPER)
+    _set_grads([p], 2)
+    for bad in (torch.ones(0, device=DEV), torch.ones(2, device=DEV)):
+        with pytest.raises(ValueError, match="grad_scale"):
+            opt.step(grad_scale=bad)
+    with pytest.raises(ValueError, match="grad_scale"):
+        opt.step(grad_scale=0.5)
+    assert opt.state_dict()["state"][0]["step"] == 0
+    opt.step(grad_scale=torch.ones(1, dtype=torch.float64, device=DEV))
+
+
 def test_a_step_that_raises_does_not_count():
     (p,) = _params([(30,)], torch.float32, 1)
     opt = mhc_b200.AdamW([p], **HYPER)
