@@ -53,7 +53,8 @@ def _apart(params) -> bool:
 
 class _States(dict):
     """Optimizer.state: a parameter's views of the flat buffers are made when they are
-    first asked for (hundreds of parameters, four buffers each)."""
+    first asked for (hundreds of parameters, four buffers each), those of all when the
+    state is walked."""
 
     def __init__(self, owner):
         super().__init__()
@@ -65,6 +66,31 @@ class _States(dict):
         pack, i = self.where[p]
         self[p] = pack.state_of(i)
         return self[p]
+
+    def _all(self):
+        self.where = self.owner._where()
+        return [(p, self[p]) for p in self.where]
+
+    def __len__(self):
+        return len(self.owner._where())
+
+    def __contains__(self, p):
+        return p in self.owner._where()
+
+    def __iter__(self):
+        return iter(self.owner._where())
+
+    def keys(self):
+        return self.owner._where().keys()
+
+    def values(self):
+        return [s for _, s in self._all()]
+
+    def items(self):
+        return self._all()
+
+    def get(self, p, default=None):
+        return self[p] if p in self else default
 
 
 class _Pack:
@@ -314,6 +340,8 @@ class AdamW(torch.optim.Optimizer):
                 for i, p in enumerate(pack.params)}
 
     def state_dict(self) -> dict:
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         where, state, groups, k = self._where(), {}, [], 0
         for g in self.param_groups:
             ids = list(range(k, k + len(g["params"])))
@@ -322,11 +350,19 @@ class AdamW(torch.optim.Optimizer):
             for i, p in zip(ids, g["params"]):
                 pack, at = where[p]
                 state[i] = {"step": pack.steps[at], **pack.state_of(at)}
-        return {"state": state, "param_groups": groups, "state_bits": self.state_bits,
-                "seed": self.seed}
+        saved = {"state": state, "param_groups": groups, "state_bits": self.state_bits,
+                 "seed": self.seed}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            other = hook(self, saved)
+            saved = saved if other is None else other
+        return saved
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
+        state_dict = dict(state_dict)  # a hook may change it
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            other = hook(self, state_dict)
+            state_dict = state_dict if other is None else other
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("loaded state dict has other parameter groups")
@@ -355,3 +391,5 @@ class AdamW(torch.optim.Optimizer):
         self.seed = int(state_dict["seed"])
         for g, s in zip(self.param_groups, groups):
             g.update({n: v for n, v in s.items() if n != "params"})
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)

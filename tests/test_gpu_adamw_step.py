@@ -222,3 +222,38 @@ def test_8_bit_state_of_another_layout_is_refused():
     d = torch.nn.Parameter(torch.zeros(8, 1, device=DEV))
     oc, od = (mhc_b200.AdamW([x], state_bits=8) for x in (c, d))
     od.load_state_dict(oc.state_dict())
+
+
+def test_state_hooks_and_walks():
+    params = _params([(30,), (4, 4)], torch.float32, 1)
+    opt = mhc_b200.AdamW(params, **HYPER)
+    assert len(opt.state) == 2 and list(opt.state) == params and params[0] in opt.state
+    assert [s["exp_avg"].shape for s in opt.state.values()] == [p.shape for p in params]
+    assert all(s is opt.state[p] for p, s in opt.state.items())
+    _set_grads(params, 2)
+    opt.step()
+    seen = []
+    opt.register_state_dict_pre_hook(lambda o: seen.append("pre"))
+
+    def post(o, d):
+        seen.append("post")
+        d["note"] = 5
+
+    opt.register_state_dict_post_hook(post)
+    opt.register_state_dict_post_hook(lambda o, d: {**d, "other": 6})
+    saved = opt.state_dict()
+    assert seen == ["pre", "post"] and saved["note"] == 5 and saved["other"] == 6
+    new = mhc_b200.AdamW(_params([(30,), (4, 4)], torch.float32, 9))
+
+    def before(o, d):
+        seen.append("before")
+        d = {**d, "param_groups": [{**g, "lr": 0.125} for g in d["param_groups"]]}
+        return d
+
+    new.register_load_state_dict_pre_hook(before)
+    new.register_load_state_dict_post_hook(lambda o: seen.append(("after", o.param_groups[0]["lr"])))
+    new.load_state_dict(saved)
+    assert seen == ["pre", "post", "before", ("after", 0.125)]
+    assert saved["param_groups"][0]["lr"] == HYPER["lr"]
+    for a, b in zip(opt.state.values(), new.state.values()):
+        assert torch.equal(a["exp_avg"], b["exp_avg"])
