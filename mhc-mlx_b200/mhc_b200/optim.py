@@ -100,20 +100,16 @@ class _Pack:
         self.params, self.bits, self.salt = params, bits, salt
         self.dtype, self.device = params[0].dtype, params[0].device
         self.steps = [0] * len(params)
-        n = len(params)
         sizes = [p.numel() for p in params]
         offsets = [0]
         for s in sizes:
             offsets.append(offsets[-1] + -(-s // BLOCK) * BLOCK)
         total = offsets.pop()
-        self.offsets, self.total = offsets, total
-        self.numel = (ctypes.c_int64 * n)(*sizes)
-        self.off = (ctypes.c_int64 * n)(*offsets)
+        self.sizes, self.offsets, self.total = sizes, offsets, total
+        self._arrays()
         # every gradient must lie in memory as its parameter does
         self.plain = all(p.is_contiguous() for p in params)
         self.strides = [p.stride() for p in params]
-        # written by each step's look at the parameters, read by its launch
-        self.p_ptr, self.g_ptr = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)()
         self.code, self.where = C.dtype_code(self.dtype), params[0].get_device()
         zeros = lambda k, dt: torch.zeros(max(k, 1), dtype=dt, device=self.device)[:k]  # noqa: E731
         f8, f32 = torch.float8_e4m3fn, torch.float32
@@ -131,6 +127,27 @@ class _Pack:
             self.buffers["master"] = zeros(total, f32)
             for p, o in zip(params, offsets):
                 self.view("master", p, o).copy_(p.detach())
+
+    def _arrays(self) -> None:
+        n = len(self.sizes)
+        self.numel = (ctypes.c_int64 * n)(*self.sizes)
+        self.off = (ctypes.c_int64 * n)(*self.offsets)
+        # written by each step's look at the parameters, read by its launch
+        self.p_ptr, self.g_ptr = (ctypes.c_uint64 * n)(), (ctypes.c_uint64 * n)()
+
+    def __getstate__(self) -> dict:
+        arrays = ("numel", "off", "p_ptr", "g_ptr")
+        state = {k: v for k, v in self.__dict__.items() if k not in arrays}
+        # 8-bit floats go as bytes: pickle does not know them
+        state["buffers"] = {k: b.view(torch.uint8) if b.dtype == torch.float8_e4m3fn else b
+                            for k, b in self.buffers.items()}
+        return state
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self.buffers = {k: b.view(torch.float8_e4m3fn) if b.dtype == torch.uint8 else b
+                        for k, b in state["buffers"].items()}
+        self._arrays()
 
     def view(self, key: str, p: torch.Tensor, offset: int) -> torch.Tensor:
         """p's part of a buffer, laid out as p is; of a scale, its blocks."""
@@ -328,8 +345,12 @@ class AdamW(torch.optim.Optimizer):
                 pack.steps = [int(step)] * len(pack.params)
 
     # ----------------------------------------------------- save and resume --
-    def __getstate__(self) -> dict:  # copies and pickles: all but the views, made on use
-        return {k: v for k, v in self.__dict__.items() if k != "state"}
+    def __getstate__(self) -> dict:
+        """For copies and pickles: what the class keeps, but for the views, which are made
+        on use.  Not what others have hung on this instance: a scheduler's wrapped ``step``
+        would go on stepping the original."""
+        return {k: self.__dict__[k] for k in ("defaults", "param_groups", "state_bits",
+                                              "master_weights", "seed", "_packs")}
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)

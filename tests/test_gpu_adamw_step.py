@@ -3,7 +3,9 @@ types' ranges.  Tolerances as in test_gpu_adamw.py."""
 
 from __future__ import annotations
 
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -257,3 +259,43 @@ def test_state_hooks_and_walks():
     assert saved["param_groups"][0]["lr"] == HYPER["lr"]
     for a, b in zip(opt.state.values(), new.state.values()):
         assert torch.equal(a["exp_avg"], b["exp_avg"])
+
+
+def test_a_copy_with_a_scheduler_steps_its_own_parameters():
+    (p,) = _params([(300,)], torch.float32, 1)
+    opt = mhc_b200.AdamW([p], **HYPER)
+    schedule = torch.optim.lr_scheduler.LambdaLR(opt, lambda n: 0.5 ** n)
+    _set_grads([p], 2)
+    opt.step()
+    schedule.step()
+    twin = copy.deepcopy(opt)
+    (q,) = twin.param_groups[0]["params"]
+    q.grad = p.grad.clone()
+    before = p.detach().clone()
+    twin.step()
+    assert torch.equal(p.detach(), before) and not torch.equal(q.detach(), before)
+    opt.step()
+    assert torch.equal(p.detach(), q.detach())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_pickled(bits):
+    params = _params([(50, 7), (4,)], torch.bfloat16, 1) + _params([(9,)], torch.float32, 2)
+    opt = mhc_b200.AdamW([{"params": params[:2]}, {"params": params[2:], "lr": 0.5}],
+                         state_bits=bits, master_weights=True, seed=3, **HYPER)
+    torch.optim.lr_scheduler.LambdaLR(opt, lambda n: 1.0)
+    for t in range(2):
+        _set_grads(params, t)
+        opt.step()
+    twin = pickle.loads(pickle.dumps(opt))
+    own = [p for g in twin.param_groups for p in g["params"]]
+    assert all(torch.equal(p, q) and p is not q for p, q in zip(params, own))
+    assert twin.state_bits == bits and twin.seed == 3 and twin.param_groups[1]["lr"] == 0.5
+    for t in range(2, 4):
+        for ps, o in ((params, opt), (own, twin)):
+            _set_grads(ps, t)
+            o.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, own))
+    for k in (0, 1):
+        for a, b in zip(opt.state_buffers(k).values(), twin.state_buffers(k).values()):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
