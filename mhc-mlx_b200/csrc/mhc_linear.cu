@@ -684,8 +684,10 @@ int gemm(const char* fn, const Matrix& a, const Matrix& b, const Epilogue<T>& ep
 
 constexpr int kFewRows = 16;
 // Rows to a block of k_act_grad: 128, fewer (down to 16) while there are not two
-// blocks an SM.
+// blocks an SM, more where they would be more than a grid's second axis takes.
 int rows_per(int64_t M, int64_t N) {
+  constexpr int64_t kMost = 65535;
+  if (M > 128 * kMost) return (int)up8((M + kMost - 1) / kMost);
   int per = 128;
   while (per > 16 && (M + per - 1) / per * ((N + 255) / 256) < 2 * (int64_t)sm_count()) per /= 2;
   return per;
@@ -752,7 +754,6 @@ int backward(const LinearGradArg& l, cudaStream_t st) {
       part = static_cast<float*>(ws.take((size_t)parts * (size_t)l.N * sizeof(float)));
       if (!part) return no_space(fn);
     }
-    if (parts > 65535) return set_error(MHC_ERR_UNSUPPORTED, "%s: M=%lld is too large", fn, (long long)l.M);
     const dim3 grid((unsigned)((l.N + 255) / 256), (unsigned)parts);
     k_act_grad<T, ACT><<<grid, 256, 0, st>>>(static_cast<const T*>(l.dy), l.ldy, static_cast<const float*>(l.z),
                                              l.ldz, static_cast<T*>(q), up8(l.N), part, l.M, (int)l.N, per,

@@ -53,3 +53,28 @@ def test_forward_mode_is_refused():
         y = linear_act(leaf, w)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, leaf, fwAD.make_dual(dy, torch.ones_like(dy)))
+
+
+def test_more_rows_than_a_grid_has():
+    """8.4 million rows: more blocks of 128 rows than the second axis of a grid takes."""
+    M, N, K = 65535 * 128 + 77, 8, 8
+    g = torch.Generator(device=DEV).manual_seed(1)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g).to(torch.bfloat16)  # noqa: E731
+    x, w, b, dy = (t.requires_grad_(i < 3) for i, t in enumerate((r(M, K), r(N, K), r(N), r(M, N))))
+    y = linear_act(x, w, b, activation="relu")
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], dy)
+    with torch.no_grad():
+        z = x.double() @ w.double().t() + b.double()
+        size = x.double().abs() @ w.double().abs().t() + b.double().abs()
+        dz = dy.double() * (z > 0)
+        # a z that is 0 to within its error may fall on either side
+        edge = torch.where(z.abs() <= 2 * EPS * size, dy.double().abs(), torch.zeros_like(z))
+        u = U[torch.bfloat16]
+        rounded = edge + u * dz.abs()
+        for name, got, want, tol in (
+                ("dx", dx, dz @ w.double(), rounded @ w.double().abs() + EPS * (dz.abs() @ w.double().abs())),
+                ("dw", dw, dz.t() @ x.double(),
+                 rounded.t() @ x.double().abs() + EPS * (dz.abs().t() @ x.double().abs())),
+                ("db", db, dz.sum(0), edge.sum(0) + EPS * dz.abs().sum(0))):
+            _within(got, want, tol + u * want.abs() + 1e-30, name)
+    torch.cuda.empty_cache()
