@@ -5,8 +5,8 @@
 ``linear_act`` is the function, ``FusedLinear`` the module: an ``nn.Linear`` (so
 that AutoPatcher and MHCRewire take it as one) whose forward is one kernel, and
 whose backward is the input's, the weight's and the bias's gradients on the
-tensor cores.  bf16 and fp16; fp32 operands are refused, since the tensor cores
-would round them to fewer bits.
+tensor cores.  bf16 and fp16; outside torch.autocast fp32 operands are refused,
+since the tensor cores would round them to fewer bits.
 """
 
 from __future__ import annotations
@@ -42,6 +42,13 @@ def _check(x, weight, bias, residual, activation) -> int:
     return ACTIVATIONS.index(activation)
 
 
+def _autocast(*ts):
+    """The operands in the type that torch.autocast has set, as nn.Linear casts its own."""
+    to = torch.get_autocast_dtype("cuda")
+    cast = lambda t: t.is_cuda and t.is_floating_point() and t.dtype != torch.float64  # noqa: E731
+    return (t.to(to) if t is not None and cast(t) else t for t in ts)
+
+
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                residual: torch.Tensor | None = None, activation: str = "none") -> torch.Tensor:
     """act(x W^T + bias) + residual.
@@ -51,13 +58,17 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None 
     fp32, rounded once to y.  The gradients are rounded once to their tensors'
     type; with an activation the pre-activation's gradient, an operand of the
     products on the tensor cores, is rounded to the type too.  The pre-activation
-    is kept for the backward in fp32."""
+    is kept for the backward in fp32.  Under torch.autocast the operands are cast
+    to its type."""
+    if torch.is_autocast_enabled("cuda"):
+        x, weight, bias, residual = _autocast(x, weight, bias, residual)
     act = _check(x, weight, bias, residual, activation)
     return C.host().linear(x, weight, bias, residual, act)
 
 
 class FusedLinear(nn.Linear):
-    """nn.Linear with an activation, and optionally a residual, in the same kernel."""
+    """nn.Linear with an activation, and optionally a residual, in the same kernel.
+    MHCRewire calls it with one argument: wrapped, it has no residual."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True,
                  activation: str = "none", device=None, dtype=torch.bfloat16):

@@ -9,7 +9,7 @@ import torch
 import torch.autograd.forward_ad as fwAD
 from test_gpu_linear import ACT, EPS, TINY, U, _make, _within
 
-from mhc_b200 import linear_act
+from mhc_b200 import FusedLinear, linear_act
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -53,6 +53,31 @@ def test_forward_mode_is_refused():
         y = linear_act(leaf, w)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, leaf, fwAD.make_dual(dy, torch.ones_like(dy)))
+
+
+@pytest.mark.parametrize("dtype", list(U))
+def test_autocast(dtype):
+    """Under autocast the operands take its type, as nn.Linear's do."""
+    torch.manual_seed(0)
+    for own in (torch.float32, torch.bfloat16):
+        lin = FusedLinear(48, 40, activation="gelu", device=DEV, dtype=own)
+        x = torch.randn(6, 48, device=DEV, requires_grad=True)
+        r = torch.randn(6, 40, device=DEV, requires_grad=True)
+        with torch.autocast("cuda", dtype=dtype):
+            y = lin(x, residual=r)
+            like = torch.nn.Linear(48, 40, device=DEV)(x)
+        assert y.dtype == like.dtype == dtype
+        cast = [t.detach().to(dtype).requires_grad_() for t in (x, lin.weight, lin.bias, r)]
+        z = linear_act(*cast[:3], residual=cast[3], activation="gelu")
+        assert torch.equal(y, z)
+        y.float().square().sum().backward()
+        z.float().square().sum().backward()
+        for a, c in zip((x, lin.weight, lin.bias, r), cast):
+            assert a.grad.dtype == a.dtype and torch.equal(a.grad, c.grad.to(a.dtype))
+    with torch.autocast("cuda", dtype=dtype, enabled=False), pytest.raises(ValueError, match="float16 or"):
+        lin(x)
+    with torch.autocast("cuda", dtype=dtype), pytest.raises(ValueError, match="dtype"):
+        linear_act(x.double(), lin.weight)
 
 
 def test_more_rows_than_a_grid_has():
