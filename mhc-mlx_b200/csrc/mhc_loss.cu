@@ -51,9 +51,12 @@ __device__ __forceinline__ float ex2(float x) {
 // sequence's summed log probabilities would collect it token by token, so the
 // exponents that go into a sum are raised, before their rounding.  A term meets
 // it up to three times (its own exponential, its thread's and its warp's
-// rescaling, the last two exact for those that hold the maximum): 4.1e-8 each
-// leaves the sums of 4000 rows of 32000 within 3e-9 of the truth on average
-// (5.0e-8 each left them 2.6e-8 high, none 9e-8 low).
+// rescaling, the last two exact for those that hold the maximum), so what is best
+// depends on the row: 4.1e-8 each was fitted to normal logits of deviation 2, 4000
+// rows of 32000 (5.0e-8 left their sums 2.6e-8 high, none 9e-8 low).  Mean error
+// of ln S with it, at 512 to 131072 logits in fp32, bf16 and fp16: deviation 2
+// 7e-9 at most, 1 2e-8 high, 5 up to 4.5e-8 low, even over (-20, 0) up to 6.3e-8
+// high, one logit 12 above the rest 5e-9, flat rows 0.
 constexpr float kExp2Mean = 4.1e-8f * kLog2e;
 // exp of a difference a - b <= 0 of finite values, or 0 for a = -inf.
 __device__ __forceinline__ float exp_diff(float a, float b) {

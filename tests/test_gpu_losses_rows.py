@@ -150,3 +150,29 @@ def test_forward_mode_is_refused():
                      lambda: mhc_b200.policy_loss_grad(x, y, z, e)):
             with pytest.raises(RuntimeError, match="forward-mode|jvp"):
                 call()
+
+
+@pytest.mark.parametrize("V", [512, 32000, 131072])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_sums_are_not_off_in_the_mean(dtype, V):
+    """The hardware's exponential is low by 5e-8 in the mean, and a term meets up to three.
+    That is taken out of the exponents: rows like a model's logits keep half of one at most,
+    rows whose sum falls to a few terms or to one power of two, none of whose errors the
+    correction was made for, two."""
+    n = min(4096, (1 << 27) // V)
+    g = torch.Generator(device=DEV).manual_seed(V)
+    r = lambda m: torch.randn(n, m, device=DEV, generator=g)  # noqa: E731
+    y = torch.zeros(n, dtype=torch.int64, device=DEV)
+    rows = {"spread 2": (2 * r(V), 2.5e-8), "spread 1": (r(V), 1e-7), "spread 5": (5 * r(V), 1e-7),
+            "flat": (torch.full((n, V), 1.25, device=DEV), 1e-7),
+            "even": (-20 * torch.rand(n, V, device=DEV, generator=g), 1e-7),
+            "one high": (torch.cat([r(V - 1), 12 + r(1)], 1), 1e-7)}
+    for name, (x, most) in rows.items():
+        x = x.to(dtype)
+        logp, stats = _capi.host().token_logprobs(x, y, IGN)
+        got = logp.double() + stats.view(n, 4)[:, 3].double()  # with its low part
+        want = torch.cat([torch.log_softmax(x[s].double(), 1)[:, 0] for s in _chunks(n, V)])
+        off = got - want
+        # the mean's own spread, four times over
+        spread = 4 * float(off.std()) / n ** 0.5
+        assert abs(float(off.mean())) <= most + spread, (name, float(off.mean()))
