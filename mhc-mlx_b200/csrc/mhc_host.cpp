@@ -13,6 +13,7 @@
 #include <Python.h>
 
 #include <cstring>
+#include <string>
 
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -46,10 +47,23 @@ struct Library {
   decltype(&mhc_last_error) last_error;
 } lib = {};
 
+PyObject* mhc_error = nullptr;  // the package's exception for a call that failed (bind)
+
+// As the package's own calls over the C ABI: ValueError for bad arguments, MHCError for
+// the rest.  The interpreter's lock may be held or not.
 void check(int status, const char* fn) {
   if (status == MHC_OK) return;
   TORCH_CHECK_VALUE(status != MHC_ERR_INVALID, fn, ": ", lib.last_error());
-  TORCH_CHECK(false, fn, " failed (status ", status, "): ", lib.last_error());
+  const std::string text = lib.last_error();  // of this thread
+  const pybind11::gil_scoped_acquire locked;
+  PyObject* e = PyObject_CallFunction(mhc_error, "sis", fn, status, text.c_str());
+  if (e) {
+    PyErr_SetObject(mhc_error, e);
+    Py_DECREF(e);
+  }
+  python_error error;
+  error.persist();  // it may travel to another thread, from the autograd engine's
+  throw error;
 }
 void* stream_of(const Tensor& t) {
   return c10::cuda::getCurrentCUDAStream(t.device().index()).stream();
@@ -399,18 +413,19 @@ PyObject* policy(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of the entry points of Library, in their order)
+// bind(addresses of the entry points of Library, in their order, MHCError)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   constexpr int n = sizeof(Library) / sizeof(void*);
   void* p[n];
-  if (nargs != n) {
-    PyErr_Format(PyExc_TypeError, "bind: %d addresses are expected", n);
+  if (nargs != n + 1 || !PyExceptionClass_Check(args[n])) {
+    PyErr_Format(PyExc_TypeError, "bind: %d addresses and an exception are expected", n);
     return nullptr;
   }
   for (int i = 0; i < n; ++i) p[i] = PyLong_AsVoidPtr(args[i]);
   if (PyErr_Occurred()) return nullptr;
   static_assert(sizeof(Library) == sizeof(p), "one address a member");
   std::memcpy(&lib, p, sizeof(p));
+  Py_XSETREF(mhc_error, Py_NewRef(args[n]));
   Py_RETURN_NONE;
 }
 
@@ -492,7 +507,7 @@ PyCFunction fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
 }
 PyMethodDef methods[] = {
-    {"bind", fast(bind), METH_FASTCALL, "bind(the entry points' addresses)"},
+    {"bind", fast(bind), METH_FASTCALL, "bind(the entry points' addresses, MHCError)"},
     {"token_logprobs", fast(token_logprobs), METH_FASTCALL, "-> (logp, stats)"},
     {"logits_grad", fast(logits_grad), METH_FASTCALL, "-> dlogits"},
     {"preference", fast(preference), METH_FASTCALL, "-> (loss, logp, margins, dlogits, records)"},

@@ -187,7 +187,7 @@ def host():
         module.bind(*(ctypes.cast(getattr(lib, n), _P).value for n in (
             "mhc_linear_fwd_workspace_bytes", "mhc_linear_fwd", "mhc_linear_bwd_workspace_bytes",
             "mhc_linear_bwd", "mhc_token_logprobs", "mhc_logits_grad", "mhc_preference_loss",
-            "mhc_policy_workspace_bytes", "mhc_policy_loss", "mhc_last_error")))
+            "mhc_policy_workspace_bytes", "mhc_policy_loss", "mhc_last_error")), MHCError)
         _host = module
     return _host
 

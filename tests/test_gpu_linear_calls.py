@@ -4,12 +4,14 @@ fp32, so nothing is allowed for a rounding of z."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 from test_gpu_linear import ACT, EPS, TINY, U, _make, _within
 
-from mhc_b200 import FusedLinear, linear_act
+from mhc_b200 import FusedLinear, _capi, linear_act, token_logprobs
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -103,3 +105,30 @@ def test_more_rows_than_a_grid_has():
                 ("db", db, dz.sum(0), edge.sum(0) + EPS * dz.abs().sum(0))):
             _within(got, want, tol + u * want.abs() + 1e-30, name)
     torch.cuda.empty_cache()
+
+
+def test_a_call_that_fails_raises_the_packages_error():
+    """In the forward, and in the backward on the autograd engine's thread; the entry points
+    are replaced by ones that return a status, so no kernel runs."""
+    host, lib = _capi.host(), _capi.load()
+    names = ["mhc_linear_fwd_workspace_bytes", "mhc_linear_fwd", "mhc_linear_bwd_workspace_bytes",
+             "mhc_linear_bwd", "mhc_token_logprobs", "mhc_logits_grad", "mhc_preference_loss",
+             "mhc_policy_workspace_bytes", "mhc_policy_loss", "mhc_last_error"]
+    real = [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names]
+    x, w, *_ = _make(20, 24, 16, torch.bfloat16, 1)
+    x.requires_grad_(True)
+    y = linear_act(x, w)
+    logits, targets = torch.zeros(4, 8, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
+    fail = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: _capi.MHC_ERR_UNSUPPORTED)
+    fake = [ctypes.cast(fail, ctypes.c_void_p).value if "bytes" not in n and "error" not in n else a
+            for n, a in zip(names, real)]
+    host.bind(*fake, _capi.MHCError)
+    try:
+        for call, name in ((lambda: linear_act(x, w), "mhc_linear_fwd"), (y.sum().backward, "mhc_linear_bwd"),
+                           (lambda: token_logprobs(logits, targets), "mhc_token_logprobs")):
+            with pytest.raises(_capi.MHCError, match=name) as e:
+                call()
+            assert e.value.code == _capi.MHC_ERR_UNSUPPORTED
+    finally:
+        host.bind(*real, _capi.MHCError)
+    linear_act(x, w).sum().backward()
