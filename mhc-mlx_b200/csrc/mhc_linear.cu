@@ -32,12 +32,14 @@
 // tile would be empty but for 1/8 of it).  Operands whose rows do not begin on
 // 16-byte boundaries, which TMA cannot read, are copied to padded rows first.
 //
-// Measured, bf16, 8192 rows, 4096 to 11008, bias and SiLU: y 537 us,
-// dz 93, db 7, dx 493, dW 538 us (1.38 to 1.50 PFLOP/s, 0.84 to 0.91 of what a
+// Measured, bf16, 8192 rows, 4096 to 11008, bias and SiLU: y and z 551 us,
+// dz 122, db 7, dx 477, dW 521 us (1.34 to 1.55 PFLOP/s, 0.82 to 0.95 of what a
 // library product reaches in a burst).  One after the other they take 2.0 ms
-// rather than these 1.67: the products draw the power limit.  Pairs of CTAs
+// rather than these 1.68: the products draw the power limit.  Pairs of CTAs
 // sharing 256 x 256 tiles, with half the operand traffic, were no faster (551,
-// 515, 550 us).  One token of 4096 x 4096: 6 us (33.6 MB, 5.6 TB/s).
+// 515, 550 us where single ones took 537, 493, 538).  One token of 4096 x 4096 by
+// launches in a row: 7.7 us with the weights from HBM (12 layers' in turn, 33.6 MB
+// each, 4.4 TB/s), 4.8 us where L2 holds them.
 #include <math_constants.h>
 
 #include "mhc_internal.h"
@@ -48,6 +50,8 @@ namespace {
 
 enum Act { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
 
+// The fast exponential and quotient: off by some 2^-20 where |z| is ordinary, far
+// below the 16-bit rounding of what comes of them.
 template <int ACT>
 __device__ __forceinline__ float act_of(float z) {
   if constexpr (ACT == kRelu) return z < 0.f ? 0.f : z;  // keeps NaN

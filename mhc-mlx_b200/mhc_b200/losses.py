@@ -199,8 +199,8 @@ def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor, ref_logpro
 # ----------------------------------------------------------------- policy --
 class _PolicyFn(torch.autograd.Function):
     """The forward also writes the gradient for an upstream of 1, which is what
-    a loss is differentiated with; the backward checks that on the device and
-    computes it anew from the logits otherwise (a scaled loss)."""
+    an unscaled loss is differentiated with; the backward checks that on the
+    device and computes it anew from the logits otherwise."""
 
     @staticmethod
     def forward(ctx, logits, targets, old, adv, ref, lo, hi, kl_coef, inv_d, ignore_index):
@@ -234,7 +234,12 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logprobs: torch
 
     D = denominator (default: the number of tokens that count; give the whole
     batch's number where gradients are accumulated).  Without such a token the
-    loss and its gradient are 0."""
+    loss and its gradient are 0.
+
+    The gradient is written with the loss, for a loss that is differentiated as it
+    is.  One that is scaled (a GradScaler's, a weight, a division) has it computed
+    a second time in the backward: ``policy_loss_grad`` takes that scale and
+    computes it once."""
     inv_d = _check_policy(logits, targets, old_logprobs, advantages, ref_logprobs, clip_low,
                           clip_high, kl_coef, denominator)
     return PolicyResult(*_PolicyFn.apply(
